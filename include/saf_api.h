@@ -198,6 +198,62 @@ int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor
                     const float* kv_bias, int64_t kv_bias_stride_bh, float sm_scale,
                     int32_t lead_rows, void* stream);
 
+/* Training forward: saf_bsa_fwd without a bias that also stores the natural
+ * log-sum-exp of every row, lse fp32 [B*H, Sq] contiguous, for saf_bsa_bwd.
+ * Unlike saf_bsa_fwd, a row with no live key gives o = 0 and lse = -inf.
+ * sm_scale is positive and finite.  workspace (16-byte aligned, of
+ * saf_bsa_fwd_lse_workspace_bytes; 0 bytes: may be null) holds the partial
+ * rows of split lead tiles, so launches may overlap on a device.
+ * No counterpart in the reference, whose kernel has no training path
+ * (utils/block_sparse_attn_kernel.py:278-281). */
+size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, int32_t block_m, int32_t lead_rows);
+int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
+                        const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
+                        int64_t col_capacity, int32_t block_m, int32_t block_n, float sm_scale,
+                        int32_t lead_rows, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Gradient of saf_bsa_fwd_lse: with p_ij = exp(sm_scale q_i.k_j - lse_i) over
+ * the listed blocks and delta_i = do_i.o_i,
+ *   dv_j = sum_i p_ij do_i,  ds_ij = p_ij (do_i.v_j - delta_i),
+ *   dq_i = sm_scale sum_j ds_ij k_j,  dk_j = sm_scale sum_i ds_ij q_i.
+ * q, k, v, out, lse as the forward had and left them (lse rows of head
+ * b*H + h at lse_stride_bh >= Sq floats), dout the gradient of
+ * out; dq, dk, dv are written whole (rows and keys that no block lists get
+ * zeros).  p is recomputed; a listed column counts once however often its
+ * row lists it.  No atomics touch the gradients: equal inputs give equal
+ * bits.  bf16 / f16: D = 64, block sizes 64 or 128, 16-byte aligned rows.
+ * f32: D = 64 or 128, block sizes multiples of 64.  At most 16384 blocks a
+ * side.  workspace: 16-byte aligned, of saf_bsa_bwd_workspace_bytes (0 for
+ * sizes that saf_bsa_bwd refuses); calls that overlap need their own.
+ * No counterpart in the reference (utils/block_sparse_attn_kernel.py:278-281
+ * raises). */
+size_t saf_bsa_bwd_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
+                                   int32_t block_n);
+int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, const saf_tensor4* k,
+                    const saf_tensor4* v, const saf_tensor4* out, const float* lse,
+                    int64_t lse_stride_bh, const saf_tensor4* dq, const saf_tensor4* dk, const saf_tensor4* dv,
+                    const int32_t* row_ptr, const int32_t* col_idx, int64_t col_capacity,
+                    int32_t block_m, int32_t block_n, float sm_scale, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* ---- rotary positions -------------------------------------------------
+ * out[b, h, s] = x[b, h, s] for s < text_len; for the others the first
+ * rotary_dim (even) channels are rotated by table row s - text_len,
+ *   a' = a cos - b sin,  b' = b cos + a sin,
+ * over the pairs (2m, 2m + 1), or (m, m + rotary_dim / 2) with half_layout,
+ * and the rest is copied.  inverse rotates back (-sin): the gradient of the
+ * rotation, and its inverse where cos^2 + sin^2 = 1.  cos_table / sin_table:
+ * fp32 [S - text_len, rotary_dim / 2] contiguous rows, one per batch row at
+ * table_stride_b elements (0: shared).  q and k in one launch (k and out_k
+ * null: q alone); they share B, S, D and type, not H.  out may be the input
+ * itself.  Any head dim, bf16 / f16 / f32, fp32 arithmetic.
+ * No counterpart in the reference: its processors take q and k rotated. */
+int32_t saf_rope(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* out_q,
+                 const saf_tensor4* out_k, const float* cos_table, const float* sin_table,
+                 int64_t table_stride_b, int64_t text_len, int32_t rotary_dim, int32_t half_layout,
+                 int32_t inverse, void* stream);
+
 /* saf_bsa_fwd with per-query-row key intervals: row_ranges (nullable,
  * 16-byte aligned int32 [Sq, 4], shared by every head) limits the keys of
  * query row r to [x, y) U [z, w); keys outside are masked like keys past

@@ -1,0 +1,511 @@
+// bsa_bwd.cu -- gradient of block-sparse attention: entry points, the
+// preparation launch (row statistics and per-tile block lists) and the
+// CUDA-core gradient kernel.  Formulas and work split: bsa_bwd.cuh.
+#include "bsa_bwd.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace saf {
+namespace {
+
+constexpr int kT = 64;            // sub-tile edge of the CUDA-core kernel
+constexpr int kGroup = 32;        // mask lines one list block handles
+constexpr int kRowChunk = 128;    // rows one statistics block handles
+constexpr int kMaxBlocks = 16384; // 14-bit block indexes in the lists
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Mask lines that share a tile: 64-token blocks pair up under the 16-bit kernel.
+int merge_of(int32_t dtype, int block) { return dtype != SAF_F32 && block == 64 ? 2 : 1; }
+
+BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, uint8_t* base) {
+  BwdWorkspace w{};
+  const int64_t BH = q->B * q->H;
+  const int64_t nbq = (q->S + bm - 1) / bm, nbk = (k->S + bn - 1) / bn;
+  const int mq = merge_of(q->dtype, bm), mk = merge_of(q->dtype, bn);
+  w.Sp = (q->S + 127) / 128 * 128;
+  w.lines_q = static_cast<int>((nbq + mq - 1) / mq);
+  w.lines_k = static_cast<int>((nbk + mk - 1) / mk);
+  w.cap_q = static_cast<int>((nbk + 7) / 8 * 8);
+  w.cap_k = static_cast<int>((nbq + 7) / 8 * 8);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* ptr = base + at;
+    at = (at + bytes + 255) / 256 * 256;
+    return ptr;
+  };
+  w.stat_lse = reinterpret_cast<float*>(take(static_cast<size_t>(BH * w.Sp) * 4));
+  w.stat_delta = reinterpret_cast<float*>(take(static_cast<size_t>(BH * w.Sp) * 4));
+  w.list_q = reinterpret_cast<uint16_t*>(take(static_cast<size_t>(BH * w.lines_q) * w.cap_q * 2));
+  w.list_k = reinterpret_cast<uint16_t*>(take(static_cast<size_t>(BH * w.lines_k) * w.cap_k * 2));
+  w.count_q = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_q) * 4));
+  w.count_k = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_k) * 4));
+  w.bytes = at;
+  return w;
+}
+
+// ---------------------------------------------------------------------------
+// Preparation: one launch of list blocks and statistics blocks.
+// ---------------------------------------------------------------------------
+
+struct PrepParams {
+  const void* out;
+  const void* dout;
+  int64_t o_sb, o_sh, o_ss, d_sb, d_sh, d_ss;
+  int H, Sq, D;
+  const float* lse;
+  int64_t lse_stride;  // per head
+  float lse_factor;  // log2(e) for the 16-bit kernel, 1 for the fp32 kernel
+  int nbq, nbk, merge_q, merge_k;
+  int groups_q, groups_k;
+  const int32_t* row_ptr;
+  const int32_t* col_idx;
+  int64_t col_capacity;
+  BwdWorkspace w;
+  unsigned int* status;
+};
+
+// The lists of 32 mask rows or columns of head g: a bitmap of the live blocks
+// of each line, filled by one thread per listed entry and read back ascending.
+// A line with an entry outside the mask sets the bad-index flag and skips it.
+__device__ void build_lists(const PrepParams& p, int g, int group, bool columns) {
+  extern __shared__ uint32_t sm[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int other = columns ? p.nbq : p.nbk, words = (other + 31) >> 5;
+  uint32_t* bits = sm;                                       // [32][words]
+  int32_t* rp = reinterpret_cast<int32_t*>(sm + kGroup * words);  // [rows + 1]
+  const int line0 = group * kGroup;
+  const int row0 = columns ? 0 : line0;
+  const int rows = columns ? p.nbq : min(kGroup, p.nbq - line0);
+  for (int i = tid; i < kGroup * words; i += blockDim.x) bits[i] = 0u;
+  const int32_t* src = p.row_ptr + static_cast<int64_t>(g) * (p.nbq + 1) + row0;
+  for (int i = tid; i <= rows; i += blockDim.x) {
+    const int32_t x = src[i];
+    rp[i] = x < 0 ? 0 : (static_cast<int64_t>(x) > p.col_capacity ? static_cast<int32_t>(p.col_capacity) : x);
+  }
+  __syncthreads();
+  for (int e = rp[0] + tid; e < rp[rows]; e += blockDim.x) {
+    int lo = 0, hi = rows;  // the row whose range holds entry e
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (rp[mid] <= e)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int c = p.col_idx[e];
+    if (c < 0 || c >= p.nbk) {
+      atomicOr(p.status, SAF_DEV_BADINDEX);
+      continue;
+    }
+    const int line = columns ? c - line0 : lo, bit = columns ? row0 + lo : c;
+    if (line >= 0 && line < kGroup) atomicOr(&bits[line * words + (bit >> 5)], 1u << (bit & 31));
+  }
+  __syncthreads();
+  const int merge = columns ? p.merge_k : p.merge_q;
+  const int lines = columns ? p.w.lines_k : p.w.lines_q, cap = columns ? p.w.cap_k : p.w.cap_q;
+  uint16_t* list = columns ? p.w.list_k : p.w.list_q;
+  int32_t* count = columns ? p.w.count_k : p.w.count_q;
+  for (int t = warp; t < kGroup / merge; t += blockDim.x >> 5) {
+    const int tile = line0 / merge + t;
+    if (tile >= lines) break;
+    const uint32_t* ba = bits + t * merge * words;
+    const uint32_t* bb = ba + (merge - 1) * words;
+    uint16_t* dst = list + (static_cast<int64_t>(g) * lines + tile) * cap;
+    int n = 0;
+    for (int w0 = 0; w0 < words; w0 += 32) {
+      const int w = w0 + lane;
+      const uint32_t a = w < words ? ba[w] : 0u, b = w < words ? bb[w] : 0u;
+      uint32_t u = a | b;
+      int incl = __popc(u);
+      const int cnt = incl;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+      }
+      int pos = n + incl - cnt;
+      while (u != 0u) {
+        const int bit = __ffs(u) - 1;
+        u &= u - 1u;
+        const uint32_t half = ((a >> bit) & 1u) | (((b >> bit) & 1u) << 1);
+        dst[pos++] = static_cast<uint16_t>((w * 32 + bit) | (half << 14));
+      }
+      n += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) count[static_cast<int64_t>(g) * lines + tile] = n;
+  }
+}
+
+__device__ __forceinline__ float2 unpack2(uint32_t x, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t x, const __half*) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// delta and the log-sum-exp of 128 rows of head g.  A row that sees no key
+// (lse -inf) and the rows that pad the last tile get +inf, so that every
+// exp(s - lse) of theirs is 0.
+template <typename T>
+__device__ void row_stats(const PrepParams& p, int g, int chunk) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = g / p.H, h = g % p.H;
+  const T* o = static_cast<const T*>(p.out) + b * p.o_sb + h * p.o_sh;
+  const T* d = static_cast<const T*>(p.dout) + b * p.d_sb + h * p.d_sh;
+  const int64_t base = static_cast<int64_t>(g) * p.w.Sp;
+  auto store = [&](int row, float delta) {
+    const float l = row < p.Sq ? p.lse[g * p.lse_stride + row] : -INFINITY;
+    p.w.stat_lse[base + row] = l == -INFINITY ? INFINITY : l * p.lse_factor;
+    p.w.stat_delta[base + row] = l == -INFINITY ? 0.f : delta;
+  };
+  if constexpr (sizeof(T) == 2) {  // D = 64: 8 lanes of 16 bytes a row
+    const int sub = lane & 7;
+#pragma unroll
+    for (int i = 0; i < kRowChunk / 32; ++i) {
+      const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
+      float sum = 0.f;
+      if (row < p.Sq) {
+        const uint4 x = *reinterpret_cast<const uint4*>(o + row * p.o_ss + sub * 8);
+        const uint4 y = *reinterpret_cast<const uint4*>(d + row * p.d_ss + sub * 8);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 fx = unpack2(xs[e], static_cast<const T*>(nullptr));
+          const float2 fy = unpack2(ys[e], static_cast<const T*>(nullptr));
+          sum = fmaf(fx.x, fy.x, fmaf(fx.y, fy.y, sum));
+        }
+      }
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (sub == 0) store(row, sum);
+    }
+  } else {
+    for (int r = warp; r < kRowChunk; r += 8) {
+      const int row = chunk * kRowChunk + r;
+      float sum = 0.f;
+      if (row < p.Sq)
+        for (int e = lane; e < p.D; e += 32) sum = fmaf(o[row * p.o_ss + e], d[row * p.d_ss + e], sum);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      if (lane == 0) store(row, sum);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
+  const int g = blockIdx.y, x = blockIdx.x;
+  if (x < p.groups_k)
+    build_lists(p, g, x, true);
+  else if (x < p.groups_k + p.groups_q)
+    build_lists(p, g, x - p.groups_k, false);
+  else
+    row_stats<T>(p, g, x - p.groups_k - p.groups_q);
+}
+
+// ---------------------------------------------------------------------------
+// CUDA-core gradient.
+// ---------------------------------------------------------------------------
+
+struct SimtBwdParams {
+  const void *q, *k, *v, *dout;
+  void *dq, *dk, *dv;
+  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, do_sb, do_sh, do_ss;
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int H, Sq, Sk, bm, bn, tiles_k;
+  float scale, lse_unit;  // lse_unit: what stat_lse is multiplied by to give natural units
+  BwdWorkspace w;
+  int merge_q, merge_k;
+};
+
+// Rows [r0, r0 + 64) of a [S, D] view as fp32 into dst [64][D + 4]; zeros past S.
+template <typename T, int D>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t ss, int r0, int S) {
+  for (int i = threadIdx.x; i < kT * D; i += 256) {
+    const int r = i / D, d = i % D;
+    dst[r * (D + 4) + d] = r0 + r < S ? static_cast<float>(src[(r0 + r) * ss + d]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
+  return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, c))));
+}
+
+// One CTA per 64 output rows: key rows (dk and dv) for blockIdx.x < tiles_k,
+// query rows (dq) after them.  The tile's own two operands (k, v or q, do)
+// stay in shared memory; the walk brings the other two.  Thread (ty, tx) of a
+// 16 x 16 grid forms the scores of walked rows ty + 16a against own rows
+// tx + 16c, then owns output rows ty*4..+3, channels tx*4..+3 (twice at D = 128).
+template <typename T, int D, bool kKeys>
+__device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
+  constexpr int LD = D + 4, DC = D / 64;
+  extern __shared__ float smf[];
+  float* a1 = smf;               // own k or q
+  float* a2 = a1 + kT * LD;      // own v or do
+  float* b1 = a2 + kT * LD;      // walked q or k
+  float* b2 = b1 + kT * LD;      // walked do or v
+  float* ps = b2 + kT * LD;      // [walked row][own row] p
+  float* ds = ps + kT * (kT + 4);
+  float* sl = ds + kT * (kT + 4);  // [64] lse of the tile's or the walked query rows
+  float* sd = sl + kT;             // [64] delta
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int b = g / p.H, h = g % p.H;
+  const T* qg = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
+  const T* kg = static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh;
+  const T* vg = static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh;
+  const T* dg = static_cast<const T*>(p.dout) + b * p.do_sb + h * p.do_sh;
+  const int own0 = tile * kT;
+  const float* lse_g = p.w.stat_lse + static_cast<int64_t>(g) * p.w.Sp;
+  const float* delta_g = p.w.stat_delta + static_cast<int64_t>(g) * p.w.Sp;
+  load_tile<T, D>(a1, kKeys ? kg : qg, kKeys ? p.k_ss : p.q_ss, own0, kKeys ? p.Sk : p.Sq);
+  load_tile<T, D>(a2, kKeys ? vg : dg, kKeys ? p.v_ss : p.do_ss, own0, kKeys ? p.Sk : p.Sq);
+  if (!kKeys && tid < kT) {
+    sl[tid] = lse_g[own0 + tid] * p.lse_unit;
+    sd[tid] = delta_g[own0 + tid];
+  }
+  float acc1[4][4 * DC], acc2[kKeys ? 4 : 1][4 * DC];  // dk or dq; dv
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < 4 * DC; ++c) {
+      acc1[i][c] = 0.f;
+      if (kKeys) acc2[i][c] = 0.f;
+    }
+  const int own_block = kKeys ? p.bn : p.bm, walk_block = kKeys ? p.bm : p.bn;
+  const int merge = kKeys ? p.merge_k : p.merge_q;
+  const int mask_line = own0 / own_block, line = mask_line / merge;
+  const uint32_t half = merge == 2 ? 1u << (mask_line & 1) : 3u;
+  const int lines = kKeys ? p.w.lines_k : p.w.lines_q, cap = kKeys ? p.w.cap_k : p.w.cap_q;
+  const int64_t at = static_cast<int64_t>(g) * lines + line;
+  const uint16_t* list = (kKeys ? p.w.list_k : p.w.list_q) + at * cap;
+  const int n = (kKeys ? p.w.count_k : p.w.count_q)[at];
+  const int walk_len = kKeys ? p.Sq : p.Sk;
+  for (int e = 0; e < n; ++e) {
+    const uint32_t ent = list[e];
+    if (((ent >> 14) & half) == 0) continue;
+    for (int w0 = (ent & 0x3fff) * walk_block, w1 = w0 + walk_block; w0 < w1 && w0 < walk_len; w0 += kT) {
+      __syncthreads();  // the previous step is consumed
+      load_tile<T, D>(b1, kKeys ? qg : kg, kKeys ? p.q_ss : p.k_ss, w0, walk_len);
+      load_tile<T, D>(b2, kKeys ? dg : vg, kKeys ? p.do_ss : p.v_ss, w0, walk_len);
+      if (kKeys && tid < kT) {
+        sl[tid] = lse_g[w0 + tid] * p.lse_unit;
+        sd[tid] = delta_g[w0 + tid];
+      }
+      __syncthreads();
+      float s[4][4], dp[4][4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[a][c] = dp[a][c] = 0.f;
+      for (int d = 0; d < D; d += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          x[c] = *reinterpret_cast<const float4*>(&b1[(ty + 16 * c) * LD + d]);
+          y[c] = *reinterpret_cast<const float4*>(&a1[(tx + 16 * c) * LD + d]);
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[a][c] = dot4(x[a], y[c], s[a][c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          x[c] = *reinterpret_cast<const float4*>(&b2[(ty + 16 * c) * LD + d]);
+          y[c] = *reinterpret_cast<const float4*>(&a2[(tx + 16 * c) * LD + d]);
+        }
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) dp[a][c] = dot4(x[a], y[c], dp[a][c]);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int wr = ty + 16 * a, orow = tx + 16 * c;
+          const int qi = kKeys ? wr : orow, key = kKeys ? own0 + orow : w0 + wr;
+          // keys past the end (zeros in shared memory) give nothing
+          const bool in = key < p.Sk && sl[qi] != INFINITY;
+          const float pr = in ? expf(s[a][c] * p.scale - sl[qi]) : 0.f;
+          if (kKeys) ps[wr * (kT + 4) + orow] = pr;
+          ds[wr * (kT + 4) + orow] = in ? pr * (dp[a][c] - sd[qi]) : 0.f;
+        }
+      __syncthreads();
+#pragma unroll 4
+      for (int w = 0; w < kT; ++w) {
+        const float4 m = *reinterpret_cast<const float4*>(&ds[w * (kT + 4) + ty * 4]);
+        const float mv[4] = {m.x, m.y, m.z, m.w};
+        float pv[4];
+        if (kKeys) {
+          const float4 pm = *reinterpret_cast<const float4*>(&ps[w * (kT + 4) + ty * 4]);
+          pv[0] = pm.x, pv[1] = pm.y, pv[2] = pm.z, pv[3] = pm.w;
+        }
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+          const float4 x = *reinterpret_cast<const float4*>(&b1[w * LD + dc * 64 + tx * 4]);
+          const float xv[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc1[i][dc * 4 + c] = fmaf(mv[i], xv[c], acc1[i][dc * 4 + c]);
+          if (kKeys) {
+            const float4 y = *reinterpret_cast<const float4*>(&b2[w * LD + dc * 64 + tx * 4]);
+            const float yv[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc2[i][dc * 4 + c] = fmaf(pv[i], yv[c], acc2[i][dc * 4 + c]);
+          }
+        }
+      }
+    }
+  }
+  T* o1 = kKeys ? static_cast<T*>(p.dk) + b * p.dk_sb + h * p.dk_sh : static_cast<T*>(p.dq) + b * p.dq_sb + h * p.dq_sh;
+  T* o2 = static_cast<T*>(p.dv) + b * p.dv_sb + h * p.dv_sh;
+  const int64_t o1_ss = kKeys ? p.dk_ss : p.dq_ss;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = own0 + ty * 4 + i;
+    if (row >= (kKeys ? p.Sk : p.Sq)) continue;
+#pragma unroll
+    for (int c = 0; c < 4 * DC; ++c) {
+      const int d = c / 4 * 64 + tx * 4 + c % 4;
+      o1[row * o1_ss + d] = static_cast<T>(acc1[i][c] * p.scale);
+      if (kKeys) o2[row * p.dv_ss + d] = static_cast<T>(acc2[i][c]);
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) bsa_bwd_simt_kernel(const SimtBwdParams p) {
+  if (static_cast<int>(blockIdx.x) < p.tiles_k)
+    simt_tile<T, D, true>(p, blockIdx.y, blockIdx.x);
+  else
+    simt_tile<T, D, false>(p, blockIdx.y, blockIdx.x - p.tiles_k);
+}
+
+template <typename T, int D>
+int32_t launch_simt(const SimtBwdParams& p, int tiles_q, int BH, cudaStream_t st) {
+  const int smem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
+  SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_bwd_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const dim3 grid(static_cast<unsigned>(p.tiles_k + tiles_q), static_cast<unsigned>(BH));
+  bsa_bwd_simt_kernel<T, D><<<grid, 256, smem, st>>>(p);
+  SAF_CUDA_TRY(cudaGetLastError());
+  return SAF_OK;
+}
+
+template <typename T>
+int32_t launch_prep(const PrepParams& p, int BH, cudaStream_t st) {
+  const int words = ((p.nbq > p.nbk ? p.nbq : p.nbk) + 31) / 32;
+  const int rows = p.nbq > kGroup ? p.nbq : kGroup;
+  const int smem = (kGroup * words + rows + 1) * 4;
+  SAF_CUDA_TRY(cudaFuncSetAttribute(bwd_prep_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const dim3 grid(static_cast<unsigned>(p.groups_k + p.groups_q + p.w.Sp / kRowChunk), static_cast<unsigned>(BH));
+  bwd_prep_kernel<T><<<grid, 256, smem, st>>>(p);
+  SAF_CUDA_TRY(cudaGetLastError());
+  return SAF_OK;
+}
+
+// Sizes every tensor of a gradient call has to agree on; no device access.
+int32_t check_sizes(const saf_tensor4* q, const saf_tensor4* k, int32_t bm, int32_t bn) {
+  int32_t rc;
+  if ((rc = check_tensor4(q)) != SAF_OK || (rc = check_tensor4(k)) != SAF_OK) return rc;
+  if (k->dtype != q->dtype) return SAF_ERR_DTYPE;
+  if (k->B != q->B || k->H != q->H || k->D != q->D) return SAF_ERR_SHAPE;
+  if (bm <= 0 || bn <= 0) return SAF_ERR_ARG;
+  if (q->S > 0x7fffffff || k->S > 0x7fffffff || q->B * q->H > 65535) return SAF_ERR_SHAPE;
+  if (q->dtype == SAF_F32) {
+    if (bm % kT != 0 || bn % kT != 0 || (q->D != 64 && q->D != 128)) return SAF_ERR_UNSUPPORTED;
+  } else if ((bm != 64 && bm != 128) || (bn != 64 && bn != 128) || q->D != 64) {
+    return SAF_ERR_UNSUPPORTED;
+  }
+  if ((q->S + bm - 1) / bm > kMaxBlocks || (k->S + bn - 1) / bn > kMaxBlocks) return SAF_ERR_UNSUPPORTED;
+  return SAF_OK;
+}
+
+}  // namespace
+}  // namespace saf
+
+using namespace saf;
+
+extern "C" size_t saf_bsa_bwd_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
+                                              int32_t block_n) {
+  if (check_sizes(q, k, block_m, block_n) != SAF_OK) return 0;
+  return layout(q, k, block_m, block_n, nullptr).bytes;
+}
+
+extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, const saf_tensor4* k,
+                               const saf_tensor4* v, const saf_tensor4* out, const float* lse,
+                               int64_t lse_stride_bh, const saf_tensor4* dq, const saf_tensor4* dk, const saf_tensor4* dv, const int32_t* row_ptr,
+                               const int32_t* col_idx, int64_t col_capacity, int32_t block_m, int32_t block_n,
+                               float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  int32_t rc;
+  if ((rc = check_sizes(q, k, block_m, block_n)) != SAF_OK) return rc;
+  const saf_tensor4* all[8] = {dout, q, out, dq, k, v, dk, dv};  // the first four by query, the others by key
+  for (int i = 0; i < 8; ++i) {
+    const saf_tensor4* t = all[i];
+    const saf_tensor4* ref = i < 4 ? q : k;
+    if ((rc = check_tensor4(t)) != SAF_OK) return rc;
+    if (t->dtype != q->dtype) return SAF_ERR_DTYPE;
+    if (t->B != ref->B || t->H != ref->H || t->S != ref->S || t->D != ref->D) return SAF_ERR_SHAPE;
+    if (q->dtype != SAF_F32 &&
+        ((reinterpret_cast<uintptr_t>(t->data) & 15) != 0 || t->stride_s % 8 != 0 ||
+         (t->H > 1 && t->stride_h % 8 != 0) || (t->B > 1 && t->stride_b % 8 != 0)))
+      return SAF_ERR_STRIDE;
+  }
+  if (lse == nullptr || row_ptr == nullptr || col_idx == nullptr || col_capacity < 0) return SAF_ERR_ARG;
+  if (!(sm_scale > 0.f) || sm_scale > 3.0e38f) return SAF_ERR_ARG;
+  if (lse_stride_bh < q->S) return SAF_ERR_STRIDE;
+  if (workspace == nullptr || workspace_bytes < saf_bsa_bwd_workspace_bytes(q, k, block_m, block_n))
+    return SAF_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;
+  DeviceScope dev_scope;
+  if ((rc = dev_scope.bind(q->data)) != SAF_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int BH = static_cast<int>(q->B * q->H);
+  PrepParams pp{};
+  pp.out = out->data, pp.dout = dout->data;
+  pp.o_sb = out->stride_b, pp.o_sh = out->stride_h, pp.o_ss = out->stride_s;
+  pp.d_sb = dout->stride_b, pp.d_sh = dout->stride_h, pp.d_ss = dout->stride_s;
+  pp.H = static_cast<int>(q->H), pp.Sq = static_cast<int>(q->S), pp.D = static_cast<int>(q->D);
+  pp.lse = lse;
+  pp.lse_stride = lse_stride_bh;
+  pp.lse_factor = 1.f;
+  pp.nbq = static_cast<int>((q->S + block_m - 1) / block_m);
+  pp.nbk = static_cast<int>((k->S + block_n - 1) / block_n);
+  pp.merge_q = merge_of(q->dtype, block_m), pp.merge_k = merge_of(q->dtype, block_n);
+  pp.groups_q = (pp.nbq + kGroup - 1) / kGroup, pp.groups_k = (pp.nbk + kGroup - 1) / kGroup;
+  pp.row_ptr = row_ptr, pp.col_idx = col_idx, pp.col_capacity = col_capacity;
+  pp.w = layout(q, k, block_m, block_n, static_cast<uint8_t*>(workspace));
+  pp.status = device_status_ptr();
+  if (pp.status == nullptr) return SAF_ERR_CUDA;
+  SimtBwdParams sp{};
+  sp.q = q->data, sp.k = k->data, sp.v = v->data, sp.dout = dout->data;
+  sp.dq = dq->data, sp.dk = dk->data, sp.dv = dv->data;
+  sp.q_sb = q->stride_b, sp.q_sh = q->stride_h, sp.q_ss = q->stride_s;
+  sp.k_sb = k->stride_b, sp.k_sh = k->stride_h, sp.k_ss = k->stride_s;
+  sp.v_sb = v->stride_b, sp.v_sh = v->stride_h, sp.v_ss = v->stride_s;
+  sp.do_sb = dout->stride_b, sp.do_sh = dout->stride_h, sp.do_ss = dout->stride_s;
+  sp.dq_sb = dq->stride_b, sp.dq_sh = dq->stride_h, sp.dq_ss = dq->stride_s;
+  sp.dk_sb = dk->stride_b, sp.dk_sh = dk->stride_h, sp.dk_ss = dk->stride_s;
+  sp.dv_sb = dv->stride_b, sp.dv_sh = dv->stride_h, sp.dv_ss = dv->stride_s;
+  sp.H = pp.H, sp.Sq = pp.Sq, sp.Sk = static_cast<int>(k->S);
+  sp.bm = block_m, sp.bn = block_n;
+  sp.tiles_k = static_cast<int>((k->S + kT - 1) / kT);
+  const int tiles_q = static_cast<int>((q->S + kT - 1) / kT);
+  sp.scale = sm_scale;
+  sp.lse_unit = 1.f;
+  sp.w = pp.w;
+  sp.merge_q = pp.merge_q, sp.merge_k = pp.merge_k;
+  if (q->dtype == SAF_F32) {
+    if ((rc = launch_prep<float>(pp, BH, st)) != SAF_OK) return rc;
+    return q->D == 64 ? launch_simt<float, 64>(sp, tiles_q, BH, st) : launch_simt<float, 128>(sp, tiles_q, BH, st);
+  }
+  if (q->dtype == SAF_BF16) {
+    if ((rc = launch_prep<__nv_bfloat16>(pp, BH, st)) != SAF_OK) return rc;
+    return launch_simt<__nv_bfloat16, 64>(sp, tiles_q, BH, st);
+  }
+  if ((rc = launch_prep<__half>(pp, BH, st)) != SAF_OK) return rc;
+  return launch_simt<__half, 64>(sp, tiles_q, BH, st);
+}

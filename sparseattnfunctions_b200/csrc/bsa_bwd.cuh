@@ -1,0 +1,36 @@
+// bsa_bwd.cuh -- what the two gradient kernels of block-sparse attention share:
+// the workspace layout, and the parameters of the preparation launch.
+//
+// Mathematics (c = sm_scale, over the listed blocks):
+//   p_ij  = exp(c q_i.k_j - lse_i)        dp_ij = do_i . v_j
+//   delta_i = do_i . o_i                  ds_ij = p_ij (dp_ij - delta_i)
+//   dv_j = sum_i p_ij do_i    dq_i = c sum_j ds_ij k_j    dk_j = c sum_i ds_ij q_i
+// p is recomputed from the log-sum-exp; nothing of size Sq x Sk is stored.
+// Every output tile is owned by one work item, which walks its own list of
+// blocks in ascending order: a query tile's key blocks (dq) or a key tile's
+// query blocks (dk, dv).  The products s and dp are formed in both walks
+// (7 matrix products instead of 5), and in return no gradient is accumulated
+// by atomics: equal inputs give equal bits.
+#pragma once
+
+#include "saf_common.cuh"
+
+namespace saf {
+
+// Workspace of one call.  A line is the tile of mask rows (dq) or mask columns
+// (dk, dv) of one work item: one mask block, or two where 64-token blocks fill
+// a 128-token tile of the 16-bit kernel.  Lists: [BH, lines, cap] entries
+// block index | live halves of the line << 14, ascending; counts [BH, lines].
+struct BwdWorkspace {
+  float* stat_lse;    // [BH, Sp]: lse (log2 units for the 16-bit kernel), +inf where nothing is seen
+  float* stat_delta;  // [BH, Sp]
+  uint16_t* list_q;   // dq lines -> key blocks
+  uint16_t* list_k;   // dk / dv lines -> query blocks
+  int32_t* count_q;
+  int32_t* count_k;
+  int lines_q, lines_k, cap_q, cap_k;
+  int64_t Sp;  // Sq rounded up to 128
+  size_t bytes;
+};
+
+}  // namespace saf

@@ -16,8 +16,9 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
                       const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                       int64_t col_capacity, int bm, int bn, const float* kv_bias,
                       int64_t bias_stride, float sm_scale, int lead_tiles, const int32_t* row_ranges,
-                      const FrameMaskArgs* frames, const PoolArgs* pool,
+                      const FrameMaskArgs* frames, const PoolArgs* pool, const TrainArgs* train,
                       cudaStream_t stream);
+int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t lead_tiles, int64_t* part_bytes);
 int32_t bsa_fwd_sm100_keys(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                            const saf_tensor4* o, const int32_t* key_list, int32_t key_len,
                            const int32_t* key_batch, float sm_scale, cudaStream_t stream);
@@ -42,6 +43,7 @@ struct SimtParams {
   float scale;
   unsigned int* status;
   const int4* row_ranges;  // nullable [Sq]: key intervals [x, y) U [z, w) of each query row
+  float* lse;  // nullable [B*H, Sq]: row log-sum-exp; rows without a live key then give zeros
 };
 
 // grid (ceil(Sq/64), B*H), 256 threads.  Thread (ty, tx) in a 16 x 16 grid
@@ -195,7 +197,10 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
   for (int i = 0; i < 4; ++i) {
     const int row = q0 + ty * 4 + i;
     if (row >= p.Sq) continue;
-    const float inv = 1.f / l_run[i];  // 0 -> inf -> NaN output, as the reference
+    const bool empty = p.lse != nullptr && l_run[i] == 0.f;
+    const float inv = empty ? 0.f : 1.f / l_run[i];  // 0 -> inf -> NaN output, as the reference
+    if (p.lse != nullptr && tx == 0)
+      p.lse[static_cast<int64_t>(g) * p.Sq + row] = empty ? -INFINITY : m_run[i] + logf(l_run[i]);
     float* og = p.o + b * p.o_sb + h * p.o_sh + static_cast<int64_t>(row) * p.o_ss;
 #pragma unroll
     for (int c = 0; c < DC; ++c) og[tx * DC + c] = acc[i][c] * inv;
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
 int32_t bsa_fwd_simt(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                      const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                      int64_t col_capacity, int bm, int bn, const float* kv_bias,
-                     int64_t bias_stride, float sm_scale, const int32_t* row_ranges,
+                     int64_t bias_stride, float sm_scale, const int32_t* row_ranges, float* lse,
                      cudaStream_t stream) {
   if (bm % kT != 0 || bn % kT != 0) return SAF_ERR_UNSUPPORTED;
   if (q->D != 64 && q->D != 128) return SAF_ERR_UNSUPPORTED;
@@ -232,6 +237,7 @@ int32_t bsa_fwd_simt(const saf_tensor4* q, const saf_tensor4* k, const saf_tenso
   p.bias_stride = bias_stride;
   p.scale = sm_scale;
   p.row_ranges = reinterpret_cast<const int4*>(row_ranges);
+  p.lse = lse;
   p.status = device_status_ptr();
   if (p.status == nullptr) return SAF_ERR_CUDA;
   dim3 grid(static_cast<unsigned>((q->S + kT - 1) / kT), static_cast<unsigned>(q->B * q->H));
@@ -264,13 +270,14 @@ int32_t check_operand(const saf_tensor4* t, const saf_tensor4* ref) {
 using namespace saf;
 
 // Validation and dispatch shared by the attention entry points; `pool`
-// (16-bit path only) asks for the pooled attention map.
+// (16-bit path only) asks for the pooled attention map, `lse` for the training
+// forward's row log-sum-exp.
 int32_t bsa_fwd_entry(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                       const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                       int64_t col_capacity, int32_t block_m, int32_t block_n, const float* kv_bias,
                       int64_t kv_bias_stride_bh, float sm_scale, int32_t lead_rows,
                       const int32_t* row_ranges, const FrameMaskArgs* frames, const PoolArgs* pool,
-                      void* stream) {
+                      const TrainArgs* train, void* stream) {
   int32_t rc = check_tensor4(q);
   if (rc != SAF_OK) return rc;
   if ((rc = check_operand(k, q)) != SAF_OK) return rc;
@@ -299,7 +306,7 @@ int32_t bsa_fwd_entry(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
     DeviceScope dev_scope;
     if ((rc = dev_scope.bind(q->data)) != SAF_OK) return rc;
     return bsa_fwd_simt(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, kv_bias,
-                        kv_bias_stride_bh, sm_scale, row_ranges, st);
+                        kv_bias_stride_bh, sm_scale, row_ranges, train != nullptr ? train->lse : nullptr, st);
   }
   // 16-bit path: tcgen05 kernel; tiles of 64 or 128, 16-byte aligned rows.
   if ((block_m != 64 && block_m != 128) || (block_n != 64 && block_n != 128))
@@ -318,7 +325,7 @@ int32_t bsa_fwd_entry(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
   return bsa_fwd_sm100(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, kv_bias,
                        kv_bias_stride_bh, sm_scale,
                        static_cast<int>(lead_tiles < 65535 ? lead_tiles : 65535), row_ranges,
-                       frames, pool, st);
+                       frames, pool, train, st);
 }
 
 extern "C" int32_t saf_bsa_fwd_ranges(const saf_tensor4* q, const saf_tensor4* k,
@@ -329,7 +336,7 @@ extern "C" int32_t saf_bsa_fwd_ranges(const saf_tensor4* q, const saf_tensor4* k
                                       float sm_scale, int32_t lead_rows, const int32_t* row_ranges,
                                       void* stream) {
   return bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, kv_bias,
-                       kv_bias_stride_bh, sm_scale, lead_rows, row_ranges, nullptr, nullptr, stream);
+                       kv_bias_stride_bh, sm_scale, lead_rows, row_ranges, nullptr, nullptr, nullptr, stream);
 }
 
 extern "C" int32_t saf_bsa_fwd_frames(const saf_tensor4* q, const saf_tensor4* k,
@@ -341,7 +348,7 @@ extern "C" int32_t saf_bsa_fwd_frames(const saf_tensor4* q, const saf_tensor4* k
                                       void* stream) {
   const FrameMaskArgs fm{frame_bits, text_len, frame_len, frames};
   return bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, nullptr, 0,
-                       sm_scale, lead_rows, nullptr, &fm, nullptr, stream);
+                       sm_scale, lead_rows, nullptr, &fm, nullptr, nullptr, stream);
 }
 
 extern "C" int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
@@ -351,6 +358,44 @@ extern "C" int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const
                                float sm_scale, int32_t lead_rows, void* stream) {
   return saf_bsa_fwd_ranges(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, kv_bias,
                             kv_bias_stride_bh, sm_scale, lead_rows, nullptr, stream);
+}
+
+static int64_t lead_tiles_of(int32_t lead_rows, int32_t block_m) {
+  return (static_cast<int64_t>(lead_rows) * block_m + 127) / 128;
+}
+
+extern "C" size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, int32_t block_m, int32_t lead_rows) {
+  if (check_tensor4(q) != SAF_OK || block_m <= 0 || lead_rows < 0 || q->dtype == SAF_F32) return 0;
+  int64_t part;
+  return static_cast<size_t>(bsa_train_split_bytes(q->B * q->H, q->S, lead_tiles_of(lead_rows, block_m), &part));
+}
+
+extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
+                                   const saf_tensor4* o, const int32_t* row_ptr,
+                                   const int32_t* col_idx, int64_t col_capacity, int32_t block_m,
+                                   int32_t block_n, float sm_scale, int32_t lead_rows, float* lse,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  int32_t rc = check_tensor4(q);
+  if (rc != SAF_OK) return rc;
+  if (lse == nullptr || !(sm_scale > 0.f) || sm_scale > 3.0e38f) return SAF_ERR_ARG;
+  if (block_m <= 0 || lead_rows < 0) return SAF_ERR_ARG;
+  for (const saf_tensor4* t : {k, v, o})
+    if ((rc = check_operand(t, q)) != SAF_OK) return rc;
+  TrainArgs train{lse, nullptr, nullptr};
+  if (q->dtype != SAF_F32) {
+    DeviceScope dev_scope;
+    if ((rc = dev_scope.bind(q->data)) != SAF_OK) return rc;
+    int64_t part = 0;
+    const int64_t need = bsa_train_split_bytes(q->B * q->H, q->S, lead_tiles_of(lead_rows, block_m), &part);
+    if (need > 0) {
+      if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) return SAF_ERR_WORKSPACE;
+      if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;
+      train.split_part = static_cast<float*>(workspace);
+      train.split_cnt = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + part);
+    }
+  }
+  return bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, nullptr, 0,
+                       sm_scale, lead_rows, nullptr, nullptr, nullptr, &train, stream);
 }
 
 extern "C" int32_t saf_bsa_fwd_keys(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,

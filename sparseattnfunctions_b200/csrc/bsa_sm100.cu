@@ -110,6 +110,7 @@ struct BsaParams {
   float* pool_scratch;  // [grid][2][list_cap][128] block maxima of each CTA's last two tiles
   float* pool_out;      // [B*H, nbp, nbk], zeroed: per-row block maxima pooled by atomic max
   int pool_block, nbp;
+  float* lse;  // training mode: natural log-sum-exp of every row, [B*H, Sq]
   // persistent schedule: query tiles per head, heads, and this launch's
   // [next tile, CTAs done] counters (zero on entry; the last CTA resets them)
   int n_tiles, BH;
@@ -285,6 +286,9 @@ constexpr int kMaskNone = 0, kMaskRanges = 1, kMaskFrames = 2;
 constexpr int kMaskKeys = 3;
 // Attention with a pooled map (no mask besides the ragged tail).
 constexpr int kMaskPool = 4;
+// Training forward (no mask besides the ragged tail): the row log-sum-exp is
+// stored too, and a row without a live key gives zeros and -inf instead of NaN.
+constexpr int kMaskTrain = 5;
 
 // TMA gather4: four rows (coordinates r0..r3 of a 2-D map whose box is one
 // row of 64 elements) into 4 x 128 bytes of shared memory, 128-byte swizzle
@@ -966,6 +970,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 #else
       constexpr bool kGuard = false;
 #endif
+      // The training mode keeps f16 P inside the type's range (65504): its
+      // rows move their max once a block sum passes 2^15.
+      constexpr float kGuardMax = kMask == kMaskTrain && !kBF16 ? 32768.f : 1.8446744e19f;
       if (spec) {
         if (!exp_pass(-m_run, !kGuard, false)) {
           ok = false;
@@ -976,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       bool upd;
       if (kGuard && spec) {
-        upd = !(lo2(rs) + hi2(rs) <= 1.8446744e19f);  // 2^64; catches inf and NaN too
+        upd = !(lo2(rs) + hi2(rs) <= kGuardMax);  // 2^64; catches inf and NaN too
         if (__any_sync(0xffffffffu, upd)) mx = block_max() * sl2;
       } else {
         mx *= sl2;
@@ -1026,7 +1033,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                    mbar_wait(bar_pv_full, (jbase + j - 1) & 1, abort_flag, p.status, p.budget_ns));
     if (have_o) tc_fence_after();
     const int qrow = q0 + row;
+    constexpr bool kTrain = kMask == kMaskTrain;
+    const bool empty = kTrain && l_run == 0.f;  // no live key: zeros, log-sum-exp -inf
     const float inv_l = 1.f / l_run;
+    // the row's log-sum-exp from a maximum in log2 units and the sum taken against it
+    auto store_lse = [&](float m, float l) {
+      p.lse[static_cast<int64_t>(g) * p.Sq + qrow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    };
     if constexpr (kPool) {
       // hand the tile's row statistics to the pool reducer (warps 2-3); a
       // row past Sq or with no visible key pools nothing
@@ -1103,11 +1116,17 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
         *cnt = 0;
-        // no visible key in any share: 0 / 0 = NaN, as the unsplit path
-        if (ok && !*abort_flag && qrow < p.Sq) store_row(acc, 1.f / ll);
+        // no visible key in any share: 0 / 0 = NaN, as the unsplit path (the
+        // sums of such a row are zeros, so scaling by 1 keeps them)
+        if (ok && !*abort_flag && qrow < p.Sq) {
+          store_row(acc, kTrain && ll == 0.f ? 1.f : 1.f / ll);
+          if constexpr (kTrain) store_lse(mm, ll);
+        }
       }
     } else {
     const bool write = (j == 0 || have_o) && ok && !*abort_flag && qrow < p.Sq;
+    if constexpr (kTrain)
+      if (write) store_lse(m_run, l_run);
 #pragma unroll
     for (int c = 0; c < kD / 32; ++c) {
       uint32_t orr[32];
@@ -1125,8 +1144,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           uint32_t* pw = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float lo = __uint_as_float(orr[v * 8 + 2 * e]) * inv_l;
-            const float hi = __uint_as_float(orr[v * 8 + 2 * e + 1]) * inv_l;
+            const float lo = empty ? 0.f : __uint_as_float(orr[v * 8 + 2 * e]) * inv_l;
+            const float hi = empty ? 0.f : __uint_as_float(orr[v * 8 + 2 * e + 1]) * inv_l;
             pw[e] = kBF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
           }
           reinterpret_cast<uint4*>(dst)[c * 4 + v] = w;
@@ -1202,6 +1221,12 @@ int32_t split_buffers(float** part, int** cnt) {
   return SAF_OK;
 }
 
+// The most work items one lead tile may be cut into: enough to fill the
+// GPU's CTAs, at most 8.
+int split_cap(int64_t items, int sms) {
+  return static_cast<int>(std::min<int64_t>(8, (2 * sms + items - 1) / items));
+}
+
 template <int BN, bool kBias, bool kBF16, int kMask>
 int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                        BsaParams p, int n_tiles, cudaStream_t stream) {
@@ -1233,8 +1258,15 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   p.splits = 1;
   if (lead > 0 && kMask != kMaskPool && kMask != kMaskKeys) {
     const int64_t items = static_cast<int64_t>(lead) * p.BH;
-    int sp = static_cast<int>(std::min<int64_t>(8, (2 * sms + items - 1) / items));
-    if (sp > 1 && items * sp * kBM * kSplitRow <= kSplitFloats && items * kBM <= kSplitCnts) {
+    int sp = split_cap(items, sms);
+    // the training forward brings its own buffers, so that its launches may
+    // overlap (the host entry sized them by the same rule)
+    if (kMask == kMaskTrain) {
+      if (sp > 1 && p.split_part != nullptr) {
+        SAF_CUDA_TRY(cudaMemsetAsync(p.split_cnt, 0, static_cast<size_t>(items * kBM) * sizeof(int), stream));
+        p.splits = sp;
+      }
+    } else if (sp > 1 && items * sp * kBM * kSplitRow <= kSplitFloats && items * kBM <= kSplitCnts) {
       if ((rc = split_buffers(&p.split_part, &p.split_cnt)) != SAF_OK) return rc;
       SAF_CUDA_TRY(cudaMemsetAsync(p.split_cnt, 0, static_cast<size_t>(items * kBM) * sizeof(int), stream));
       p.splits = sp;
@@ -1249,12 +1281,25 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
 
 }  // namespace
 
+// Bytes of the split buffers of a training forward (0: its lead tiles run
+// unsplit): partial rows, then one counter per lead row.
+int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t lead_tiles, int64_t* part_bytes) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+    sms = 256;  // no device here: an upper bound for any sm_100 part
+  const int64_t items = std::min<int64_t>(lead_tiles, (Sq + kBM - 1) / kBM) * BH;
+  const int sp = items > 0 ? split_cap(items, sms) : 1;
+  *part_bytes = sp > 1 ? items * sp * kBM * kSplitRow * static_cast<int64_t>(sizeof(float)) : 0;
+  return sp > 1 ? *part_bytes + items * kBM * static_cast<int64_t>(sizeof(int)) : 0;
+}
+
 // Host entry for 16-bit inputs (validated by the caller in saf_api.cu).
 int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                       const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                       int64_t col_capacity, int bm, int bn, const float* kv_bias,
                       int64_t bias_stride, float sm_scale, int lead_tiles, const int32_t* row_ranges,
-                      const FrameMaskArgs* frames, const PoolArgs* pool,
+                      const FrameMaskArgs* frames, const PoolArgs* pool, const TrainArgs* train,
                       cudaStream_t stream) {
   if (q->D != kD) return SAF_ERR_UNSUPPORTED;
   if (frames != nullptr && (row_ranges != nullptr || kv_bias != nullptr)) return SAF_ERR_UNSUPPORTED;
@@ -1308,7 +1353,14 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
   const int mask = frames != nullptr ? kMaskFrames
                    : row_ranges != nullptr ? kMaskRanges
                    : pool != nullptr       ? kMaskPool
+                   : train != nullptr      ? kMaskTrain
                                            : kMaskNone;
+  if (train != nullptr) {
+    if (bias || mask != kMaskTrain) return SAF_ERR_UNSUPPORTED;
+    p.lse = train->lse;
+    p.split_part = train->split_part;
+    p.split_cnt = train->split_cnt;
+  }
   if (pool != nullptr && (bias || frames != nullptr || row_ranges != nullptr)) return SAF_ERR_UNSUPPORTED;
 #define SAF_BSA_CASE(BN_, BIAS_, BF_, MASK_)                               \
   if (bn == BN_ && bias == BIAS_ && bf16 == BF_ && mask == MASK_)          \
@@ -1333,6 +1385,10 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
   SAF_BSA_CASE(128, false, false, kMaskPool)
   SAF_BSA_CASE(64, false, true, kMaskPool)
   SAF_BSA_CASE(64, false, false, kMaskPool)
+  SAF_BSA_CASE(128, false, true, kMaskTrain)
+  SAF_BSA_CASE(128, false, false, kMaskTrain)
+  SAF_BSA_CASE(64, false, true, kMaskTrain)
+  SAF_BSA_CASE(64, false, false, kMaskTrain)
 #undef SAF_BSA_CASE
   return SAF_ERR_UNSUPPORTED;
 }

@@ -23,7 +23,7 @@ int32_t bsa_fwd_entry(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
                       int64_t col_capacity, int32_t block_m, int32_t block_n, const float* kv_bias,
                       int64_t kv_bias_stride_bh, float sm_scale, int32_t lead_rows,
                       const int32_t* row_ranges, const saf::FrameMaskArgs* frames, const saf::PoolArgs* pool,
-                      void* stream);
+                      const saf::TrainArgs* train, void* stream);
 
 namespace saf {
 namespace {
@@ -86,7 +86,7 @@ extern "C" int32_t saf_bsa_fwd_pool(const saf_tensor4* q, const saf_tensor4* k, 
   SAF_CUDA_TRY(cudaMemsetAsync(pool_out, 0, static_cast<size_t>(BH * nbp * nbk) * sizeof(float), st));
   const PoolArgs pa{scratch, pool_out, pool_block};
   rc = bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, nullptr, 0, sm_scale,
-                     lead_rows, nullptr, nullptr, &pa, stream);
+                     lead_rows, nullptr, nullptr, &pa, nullptr, stream);
   if (rc != SAF_OK) return rc;
   const int64_t rows = BH * nbp;
   pool_norm_kernel<<<static_cast<unsigned>((rows + 7) / 8), 256, 0, st>>>(pool_out, rows, static_cast<int>(nbk));

@@ -72,6 +72,15 @@ struct PoolArgs {
   int32_t pool_block;  // 64 or 128 query rows per pooled row
 };
 
+// Training forward of the attention kernels: the row log-sum-exp output
+// [B*H, Sq] and, for the 16-bit kernel, the caller's buffers for split lead
+// tiles (partial rows and row counters; null when its tiles run unsplit).
+struct TrainArgs {
+  float* lse;
+  float* split_part;
+  int* split_cnt;
+};
+
 // Common checks of a [B,H,S,D] view: non-null, D-stride 1 implied, positive
 // sizes, known dtype.
 inline int32_t check_tensor4(const saf_tensor4* t) {

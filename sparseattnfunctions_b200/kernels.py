@@ -388,6 +388,151 @@ def bsa_fwd_pool(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCS
     return out, pool
 
 
+def _check_csr(csr: BlockCSR, q: torch.Tensor, k: torch.Tensor) -> None:
+    B, H, Sq, _ = q.shape
+    if (csr.B, csr.H) != (B, H) or csr.nbq != math.ceil(Sq / csr.block_m) or \
+            csr.nbk != math.ceil(k.shape[2] / csr.block_n):
+        raise ValueError("block list does not match q/k shapes")
+    if csr.row_ptr.dtype != torch.int32 or csr.col_idx.dtype != torch.int32 or \
+            csr.row_ptr.numel() != B * H * (csr.nbq + 1) or \
+            not (csr.row_ptr.is_contiguous() and csr.col_idx.is_contiguous()):
+        raise ValueError("block list must hold contiguous int32 row_ptr [B*H, nbq + 1] and col_idx")
+
+
+def _rows_last(x: torch.Tensor, unit: int) -> torch.Tensor:
+    """``x``, copied unless its rows are whole, apart, and start at multiples of
+    ``unit`` elements: a gradient comes in whatever layout the code after an
+    operator left it (expanded, an odd offset), which the caller does not
+    choose."""
+    if x.dim() == 4 and (x.stride(3) != 1 or x.stride(2) < x.shape[3] or x.data_ptr() % (unit * x.element_size())
+                         or any(s % unit for s in x.stride()[:3])):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR, sm_scale: float,
+                out: Optional[torch.Tensor] = None):
+    """Training forward: block-sparse attention over the live blocks of
+    ``csr`` and the row log-sum-exp that ``bsa_bwd`` needs.  Returns ``(out,
+    lse)``, ``lse`` fp32 ``[B, H, Sq]`` in natural units; a row with no live
+    key gives zeros and ``-inf`` (``bsa_fwd`` gives NaN there)."""
+    dev = _require_cuda(q, k, v, csr.row_ptr, csr.col_idx)
+    q, k, v = _d_last(q), _d_last(k), _d_last(v)
+    if q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or v.shape != k.shape or \
+            k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+    B, H, Sq, D = q.shape
+    _check_csr(csr, q, k)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("out must have the shape, type and device of q")
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev)
+    if q.numel() == 0 or k.numel() == 0:  # no key at all is a row without a live key
+        return out.zero_(), lse.fill_(-math.inf)
+    lib = _lib.load()
+    tq, tk, tv, to = _t4(q), _t4(k), _t4(v), _t4(out)
+    lead = int(csr.dense_rows)
+    ws, ws_bytes = None, 0
+    if lead > 0:
+        with torch.cuda.device(dev):
+            ws_bytes = int(lib.saf_bsa_fwd_lse_workspace_bytes(ctypes.byref(tq), csr.block_m, lead))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = lib.saf_bsa_fwd_lse(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(to),
+                             csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
+                             csr.block_n, float(sm_scale), lead, lse.data_ptr(),
+                             ws.data_ptr() if ws_bytes else None, ws_bytes, _stream_ptr(dev))
+    _lib.check("saf_bsa_fwd_lse", rc)
+    return out, lse
+
+
+def bsa_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+            lse: torch.Tensor, csr: BlockCSR, sm_scale: float):
+    """Gradient of ``bsa_fwd_lse``: ``(dq, dk, dv)`` from the gradient
+    ``dout`` of its output, its inputs, and the ``out`` and ``lse`` it
+    returned.  The probabilities are recomputed block by block; rows and keys
+    that no block lists get zeros.  Equal inputs give equal bits
+    (saf_bsa_bwd)."""
+    dev = _require_cuda(dout, q, k, v, out, lse, csr.row_ptr, csr.col_idx)
+    dout = _rows_last(dout, 1 if dout.dtype == torch.float32 else 8)
+    q, k, v, out = _d_last(q), _d_last(k), _d_last(v), _d_last(out)
+    if dout.dim() != 4 or q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or v.shape != k.shape or \
+            k.shape[3] != q.shape[3] or dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"dout {tuple(dout.shape)}, q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
+                         f"out {tuple(out.shape)} do not match")
+    _check_csr(csr, q, k)
+    if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
+        raise ValueError(f"lse must be a float32 {list(q.shape[:3])} tensor")
+    if lse.stride(2) != 1 or lse.stride(1) < lse.shape[2] or lse.stride(0) != lse.shape[1] * lse.stride(1):
+        lse = lse.contiguous()
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    lib = _lib.load()
+    tq, tk = _t4(q), _t4(k)
+    ts = [_t4(x) for x in (dout, v, out, dq, dk, dv)]
+    tdo, tv, to, tdq, tdk, tdv = (ctypes.byref(t) for t in ts)
+    ws_bytes = int(lib.saf_bsa_bwd_workspace_bytes(ctypes.byref(tq), ctypes.byref(tk), csr.block_m, csr.block_n))
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+    rc = lib.saf_bsa_bwd(tdo, ctypes.byref(tq), ctypes.byref(tk), tv, to, lse.data_ptr(), lse.stride(1), tdq, tdk,
+                         tdv, csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
+                         csr.block_n, float(sm_scale), ws.data_ptr(), ws.numel(), _stream_ptr(dev))
+    _lib.check("saf_bsa_bwd", rc)
+    return dq, dk, dv
+
+
+_ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+
+
+def rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, *, text_len: int = 0,
+         layout: str = "interleaved", inverse: bool = False, out=None):
+    """Rotary positions on ``q`` and ``k`` ``[B, H, S, D]`` in one launch.
+
+    Tokens ``s < text_len`` are copied; the others have their first ``R``
+    channels rotated by row ``s - text_len`` of ``cos`` / ``sin`` (fp32
+    ``[S - text_len, R/2]``, or ``[B, S - text_len, R/2]``), over the channel
+    pairs (2m, 2m + 1) (``layout="interleaved"``) or (m, m + R/2)
+    (``"half"``).  ``inverse`` rotates back, which is also the rotation's
+    gradient.  ``k`` may have another head count, or be None.  ``out``: the
+    pair of results (q and k themselves to rotate in place).  Returns
+    ``(q', k')``, or ``q'`` when ``k`` is None (saf_rope)."""
+    given = (q,) if k is None else (q, k)
+    dev = _require_cuda(*given, cos, sin)
+    if layout not in _ROPE_LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_ROPE_LAYOUTS)}, got {layout!r}")
+    if any(x.dim() != 4 for x in given):
+        raise ValueError("q and k must be [B, H, S, D] tensors")
+    if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more than heads")
+    B, _, S, D = q.shape
+    text_len = int(text_len)
+    if not 0 <= text_len <= S:
+        raise ValueError(f"text_len {text_len} is outside [0, {S}]")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() not in (2, 3):
+        raise ValueError("cos and sin must be float32 tensors of one [tokens, R/2] or [B, tokens, R/2] shape")
+    R = 2 * cos.shape[-1]
+    if cos.shape[-2] != S - text_len or (cos.dim() == 3 and cos.shape[0] != B) or not 0 < R <= D:
+        raise ValueError(f"table {tuple(cos.shape)} does not match {S - text_len} rotated tokens of {D} channels")
+    given = tuple(_rows_last(x, 1) for x in given)
+    if out is None:
+        outs = tuple(torch.empty_like(x) for x in given)
+    else:
+        outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
+        if len(outs) != len(given) or any(o.shape != x.shape or o.dtype != x.dtype or o.device != dev
+                                          for o, x in zip(outs, given)):
+            raise ValueError("out must match q (and k) in shape, type and device")
+    if q.numel() and given[-1].numel():
+        cos, sin = cos.contiguous(), sin.contiguous()
+        ts = [_t4(x) for x in given + outs]
+        refs = [ctypes.byref(t) for t in ts]
+        tq, tk, oq, ok = refs if k is not None else (refs[0], None, refs[1], None)
+        rc = _lib.load().saf_rope(tq, tk, oq, ok, cos.data_ptr(), sin.data_ptr(),
+                                  cos.stride(0) if cos.dim() == 3 else 0, text_len, R, _ROPE_LAYOUTS[layout],
+                                  int(inverse), _stream_ptr(dev))
+        _lib.check("saf_rope", rc)
+    return outs[0] if k is None else outs
+
+
 def permute_tokens(x: torch.Tensor, perm: torch.Tensor, heads: Optional[torch.Tensor] = None,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[b, h, s] = x[b, h, perm[s]]`` for ``[B, H, S, D]`` tensors,

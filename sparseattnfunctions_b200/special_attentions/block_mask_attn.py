@@ -26,20 +26,25 @@ import math
 
 import torch
 
-from .. import _lib, kernels
+from .. import _lib, kernels, training
 from ..geometry import COGVIDEOX_2B, VideoGeometry
+from ..rope import RopeTable
 
 
 class BlockSparseAttention:
     def __init__(self, block_size: int = 128, density: float = 0.10,
                  geometry: VideoGeometry = COGVIDEOX_2B, text_dense: bool = True,
-                 sm_scale: float | None = None, check_status: bool = False):
-        """``check_status``: after every call, synchronise the device and
+                 sm_scale: float | None = None, check_status: bool = False,
+                 rope: RopeTable | None = None):
+        """``rope``: rotary table (``rope.video_rope``) that ``forward`` applies
+        to q and k before it selects blocks; None when they come rotated.
+        ``check_status``: after every call, synchronise the device and
         raise ``SafTimeoutError`` (a kernel wait ran out) or ``SafError`` (an
         index was out of range and skipped) if the device status word is
         set.  Off by default: it costs a host synchronisation per call."""
         super().__init__()
         self.check_status = check_status
+        self.rope = rope
         self.block_size = block_size
         self.density = density
         self.geometry = geometry
@@ -58,11 +63,21 @@ class BlockSparseAttention:
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-        """``out``: optional (possibly strided) ``[B, H, S, D]`` destination."""
+        """``out``: optional (possibly strided) ``[B, H, S, D]`` destination.
+        When an input requires a gradient (and gradients are enabled) the
+        result carries one to q, k and v, the block list being a constant of
+        the step; a result written into ``out`` never does."""
         scale = self.sm_scale if self.sm_scale is not None else 1.0 / math.sqrt(q.shape[-1])
-        csr = self.select(q, k)
+        if self.rope is not None:
+            q, k = training.rotary(q, k, self.rope)
+        train = out is None and torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+        with torch.no_grad():
+            csr = self.select(q, k)
         self.last_csr = csr
-        out = kernels.bsa_fwd(q, k, v, csr, scale, out=out)
+        if train:
+            out = training.sparse_attention(q, k, v, csr, scale)
+        else:
+            out = kernels.bsa_fwd(q, k, v, csr, scale, out=out)
         if self.check_status:
             _lib.raise_on_device_status(q.device.index)
         return out
