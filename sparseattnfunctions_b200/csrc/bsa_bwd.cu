@@ -1,12 +1,20 @@
 // bsa_bwd.cu -- gradient of block-sparse attention: entry points, the
-// preparation launch (row statistics and per-tile block lists) and the
-// CUDA-core gradient kernel.  Formulas and work split: bsa_bwd.cuh.
+// preparation launch (row statistics, per-tile block lists, work items) and
+// the fp32 gradient kernel on the CUDA cores (16 bits: bsa_bwd_sm100.cu).  Formulas and work split: bsa_bwd.cuh.
 #include "bsa_bwd.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace saf {
+
+float bwd_f16_p_log2_scale();
+int32_t bsa_bwd_sm100(const saf_tensor4* dout, const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
+                      const saf_tensor4* dq, const saf_tensor4* dk, const saf_tensor4* dv, int bm, int bn,
+                      float sm_scale, const BwdWorkspace& w, cudaStream_t stream);
+
 namespace {
 
 constexpr int kT = 64;            // sub-tile edge of the CUDA-core kernel
@@ -40,6 +48,13 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
   w.list_k = reinterpret_cast<uint16_t*>(take(static_cast<size_t>(BH * w.lines_k) * w.cap_k * 2));
   w.count_q = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_q) * 4));
   w.count_k = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_k) * 4));
+  if (q->dtype != SAF_F32) {
+    const int64_t n = BH * (w.lines_q + w.lines_k);
+    w.items = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(n) * kClasses * 4));
+    w.class_count = reinterpret_cast<int32_t*>(take((kClasses + 1) * 4));
+    w.next = w.class_count + kClasses;
+    w.amax = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (w.Sp / 128)) * 4));
+  }
   w.bytes = at;
   return w;
 }
@@ -55,7 +70,8 @@ struct PrepParams {
   int H, Sq, D;
   const float* lse;
   int64_t lse_stride;  // per head
-  float lse_factor;  // log2(e) for the 16-bit kernel, 1 for the fp32 kernel
+  float lse_factor, lse_shift;  // stat_lse = lse_shift - lse_factor * lse
+  int items;                    // 1: fill the work items
   int nbq, nbk, merge_q, merge_k;
   int groups_q, groups_k;
   const int32_t* row_ptr;
@@ -70,6 +86,7 @@ struct PrepParams {
 // A line with an entry outside the mask sets the bad-index flag and skips it.
 __device__ void build_lists(const PrepParams& p, int g, int group, bool columns) {
   extern __shared__ uint32_t sm[];
+  __shared__ int cls_n[kClasses], cls_at[kClasses], my_cls[kGroup], my_pos[kGroup];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int other = columns ? p.nbq : p.nbk, words = (other + 31) >> 5;
   uint32_t* bits = sm;                                       // [32][words]
@@ -78,6 +95,7 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
   const int row0 = columns ? 0 : line0;
   const int rows = columns ? p.nbq : min(kGroup, p.nbq - line0);
   for (int i = tid; i < kGroup * words; i += blockDim.x) bits[i] = 0u;
+  if (tid < kClasses) cls_n[tid] = 0;
   const int32_t* src = p.row_ptr + static_cast<int64_t>(g) * (p.nbq + 1) + row0;
   for (int i = tid; i <= rows; i += blockDim.x) {
     const int32_t x = src[i];
@@ -133,7 +151,26 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
       }
       n += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) count[static_cast<int64_t>(g) * lines + tile] = n;
+    if (lane == 0) {
+      const uint32_t id = static_cast<uint32_t>(g * lines + tile);
+      count[id] = n;
+      if (p.items) {
+        const int cls = kClasses - 1 - (n > 0 ? 31 - __clz(n) : 0);
+        my_cls[t] = cls;
+        my_pos[t] = atomicAdd(&cls_n[cls], 1);
+      }
+    }
+  }
+  if (!p.items) return;
+  // this block's items, class by class, behind those of the blocks before it
+  __syncthreads();
+  if (tid < kClasses && cls_n[tid] > 0) cls_at[tid] = atomicAdd(&p.w.class_count[tid], cls_n[tid]);
+  __syncthreads();
+  const int tile = line0 / merge + tid;
+  if (tid < kGroup / merge && tile < lines) {
+    const int64_t n_items = static_cast<int64_t>(gridDim.y) * (p.w.lines_q + p.w.lines_k);
+    p.w.items[my_cls[tid] * n_items + cls_at[my_cls[tid]] + my_pos[tid]] =
+        (columns ? 0x80000000u : 0u) | static_cast<uint32_t>(g * lines + tile);
   }
 }
 
@@ -144,9 +181,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, const __half*) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-// delta and the log-sum-exp of 128 rows of head g.  A row that sees no key
-// (lse -inf) and the rows that pad the last tile get +inf, so that every
-// exp(s - lse) of theirs is 0.
+// -delta and the negative log-sum-exp of 128 rows of head g.  A row that sees
+// no key (lse -inf) and the rows that pad the last tile get -inf, so that
+// every exp(s - lse) of theirs is 0.  f16: also the rows' largest |do|.
 template <typename T>
 __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -156,11 +193,12 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   const int64_t base = static_cast<int64_t>(g) * p.w.Sp;
   auto store = [&](int row, float delta) {
     const float l = row < p.Sq ? p.lse[g * p.lse_stride + row] : -INFINITY;
-    p.w.stat_lse[base + row] = l == -INFINITY ? INFINITY : l * p.lse_factor;
-    p.w.stat_delta[base + row] = l == -INFINITY ? 0.f : delta;
+    p.w.stat_lse[base + row] = l == -INFINITY ? -INFINITY : p.lse_shift - l * p.lse_factor;
+    p.w.stat_delta[base + row] = l == -INFINITY ? 0.f : -delta;
   };
   if constexpr (sizeof(T) == 2) {  // D = 64: 8 lanes of 16 bytes a row
     const int sub = lane & 7;
+    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kRowChunk / 32; ++i) {
       const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
@@ -174,11 +212,24 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
           const float2 fx = unpack2(xs[e], static_cast<const T*>(nullptr));
           const float2 fy = unpack2(ys[e], static_cast<const T*>(nullptr));
           sum = fmaf(fx.x, fy.x, fmaf(fx.y, fy.y, sum));
+          amax = fmaxf(amax, fmaxf(fabsf(fy.x), fabsf(fy.y)));
         }
       }
 #pragma unroll
       for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       if (sub == 0) store(row, sum);
+    }
+    if constexpr (std::is_same<T, __half>::value) {
+      __shared__ float warp_max[8];
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+      if (lane == 0) warp_max[warp] = amax;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) amax = fmaxf(amax, warp_max[i]);
+        p.w.amax[g * (p.w.Sp / kRowChunk) + chunk] = amax;
+      }
     }
   } else {
     for (int r = warp; r < kRowChunk; r += 8) {
@@ -209,22 +260,21 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
 // ---------------------------------------------------------------------------
 
 struct SimtBwdParams {
-  const void *q, *k, *v, *dout;
-  void *dq, *dk, *dv;
+  const float *q, *k, *v, *dout;
+  float *dq, *dk, *dv;
   int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss, do_sb, do_sh, do_ss;
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
   int H, Sq, Sk, bm, bn, tiles_k;
-  float scale, lse_unit;  // lse_unit: what stat_lse is multiplied by to give natural units
+  float scale;
   BwdWorkspace w;
-  int merge_q, merge_k;
 };
 
-// Rows [r0, r0 + 64) of a [S, D] view as fp32 into dst [64][D + 4]; zeros past S.
-template <typename T, int D>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t ss, int r0, int S) {
+// Rows [r0, r0 + 64) of a [S, D] view into dst [64][D + 4]; zeros past S.
+template <int D>
+__device__ __forceinline__ void load_tile(float* dst, const float* src, int64_t ss, int r0, int S) {
   for (int i = threadIdx.x; i < kT * D; i += 256) {
     const int r = i / D, d = i % D;
-    dst[r * (D + 4) + d] = r0 + r < S ? static_cast<float>(src[(r0 + r) * ss + d]) : 0.f;
+    dst[r * (D + 4) + d] = r0 + r < S ? src[(r0 + r) * ss + d] : 0.f;
   }
 }
 
@@ -237,7 +287,7 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
 // stay in shared memory; the walk brings the other two.  Thread (ty, tx) of a
 // 16 x 16 grid forms the scores of walked rows ty + 16a against own rows
 // tx + 16c, then owns output rows ty*4..+3, channels tx*4..+3 (twice at D = 128).
-template <typename T, int D, bool kKeys>
+template <int D, bool kKeys>
 __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
   constexpr int LD = D + 4, DC = D / 64;
   extern __shared__ float smf[];
@@ -247,21 +297,21 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
   float* b2 = b1 + kT * LD;      // walked do or v
   float* ps = b2 + kT * LD;      // [walked row][own row] p
   float* ds = ps + kT * (kT + 4);
-  float* sl = ds + kT * (kT + 4);  // [64] lse of the tile's or the walked query rows
-  float* sd = sl + kT;             // [64] delta
+  float* sl = ds + kT * (kT + 4);  // [64] -lse of the tile's or the walked query rows
+  float* sd = sl + kT;             // [64] -delta
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int b = g / p.H, h = g % p.H;
-  const T* qg = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
-  const T* kg = static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh;
-  const T* vg = static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh;
-  const T* dg = static_cast<const T*>(p.dout) + b * p.do_sb + h * p.do_sh;
+  const float* qg = p.q + b * p.q_sb + h * p.q_sh;
+  const float* kg = p.k + b * p.k_sb + h * p.k_sh;
+  const float* vg = p.v + b * p.v_sb + h * p.v_sh;
+  const float* dg = p.dout + b * p.do_sb + h * p.do_sh;
   const int own0 = tile * kT;
   const float* lse_g = p.w.stat_lse + static_cast<int64_t>(g) * p.w.Sp;
   const float* delta_g = p.w.stat_delta + static_cast<int64_t>(g) * p.w.Sp;
-  load_tile<T, D>(a1, kKeys ? kg : qg, kKeys ? p.k_ss : p.q_ss, own0, kKeys ? p.Sk : p.Sq);
-  load_tile<T, D>(a2, kKeys ? vg : dg, kKeys ? p.v_ss : p.do_ss, own0, kKeys ? p.Sk : p.Sq);
+  load_tile<D>(a1, kKeys ? kg : qg, kKeys ? p.k_ss : p.q_ss, own0, kKeys ? p.Sk : p.Sq);
+  load_tile<D>(a2, kKeys ? vg : dg, kKeys ? p.v_ss : p.do_ss, own0, kKeys ? p.Sk : p.Sq);
   if (!kKeys && tid < kT) {
-    sl[tid] = lse_g[own0 + tid] * p.lse_unit;
+    sl[tid] = lse_g[own0 + tid];
     sd[tid] = delta_g[own0 + tid];
   }
   float acc1[4][4 * DC], acc2[kKeys ? 4 : 1][4 * DC];  // dk or dq; dv
@@ -273,23 +323,19 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
       if (kKeys) acc2[i][c] = 0.f;
     }
   const int own_block = kKeys ? p.bn : p.bm, walk_block = kKeys ? p.bm : p.bn;
-  const int merge = kKeys ? p.merge_k : p.merge_q;
-  const int mask_line = own0 / own_block, line = mask_line / merge;
-  const uint32_t half = merge == 2 ? 1u << (mask_line & 1) : 3u;
+  const int line = own0 / own_block;
   const int lines = kKeys ? p.w.lines_k : p.w.lines_q, cap = kKeys ? p.w.cap_k : p.w.cap_q;
   const int64_t at = static_cast<int64_t>(g) * lines + line;
   const uint16_t* list = (kKeys ? p.w.list_k : p.w.list_q) + at * cap;
   const int n = (kKeys ? p.w.count_k : p.w.count_q)[at];
   const int walk_len = kKeys ? p.Sq : p.Sk;
   for (int e = 0; e < n; ++e) {
-    const uint32_t ent = list[e];
-    if (((ent >> 14) & half) == 0) continue;
-    for (int w0 = (ent & 0x3fff) * walk_block, w1 = w0 + walk_block; w0 < w1 && w0 < walk_len; w0 += kT) {
+    for (int w0 = (list[e] & 0x3fff) * walk_block, w1 = w0 + walk_block; w0 < w1 && w0 < walk_len; w0 += kT) {
       __syncthreads();  // the previous step is consumed
-      load_tile<T, D>(b1, kKeys ? qg : kg, kKeys ? p.q_ss : p.k_ss, w0, walk_len);
-      load_tile<T, D>(b2, kKeys ? dg : vg, kKeys ? p.do_ss : p.v_ss, w0, walk_len);
+      load_tile<D>(b1, kKeys ? qg : kg, kKeys ? p.q_ss : p.k_ss, w0, walk_len);
+      load_tile<D>(b2, kKeys ? dg : vg, kKeys ? p.do_ss : p.v_ss, w0, walk_len);
       if (kKeys && tid < kT) {
-        sl[tid] = lse_g[w0 + tid] * p.lse_unit;
+        sl[tid] = lse_g[w0 + tid];
         sd[tid] = delta_g[w0 + tid];
       }
       __syncthreads();
@@ -326,10 +372,10 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
           const int wr = ty + 16 * a, orow = tx + 16 * c;
           const int qi = kKeys ? wr : orow, key = kKeys ? own0 + orow : w0 + wr;
           // keys past the end (zeros in shared memory) give nothing
-          const bool in = key < p.Sk && sl[qi] != INFINITY;
-          const float pr = in ? expf(s[a][c] * p.scale - sl[qi]) : 0.f;
+          const bool in = key < p.Sk && sl[qi] != -INFINITY;
+          const float pr = in ? expf(fmaf(s[a][c], p.scale, sl[qi])) : 0.f;
           if (kKeys) ps[wr * (kT + 4) + orow] = pr;
-          ds[wr * (kT + 4) + orow] = in ? pr * (dp[a][c] - sd[qi]) : 0.f;
+          ds[wr * (kT + 4) + orow] = in ? pr * (dp[a][c] + sd[qi]) : 0.f;
         }
       __syncthreads();
 #pragma unroll 4
@@ -361,8 +407,8 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
       }
     }
   }
-  T* o1 = kKeys ? static_cast<T*>(p.dk) + b * p.dk_sb + h * p.dk_sh : static_cast<T*>(p.dq) + b * p.dq_sb + h * p.dq_sh;
-  T* o2 = static_cast<T*>(p.dv) + b * p.dv_sb + h * p.dv_sh;
+  float* o1 = kKeys ? p.dk + b * p.dk_sb + h * p.dk_sh : p.dq + b * p.dq_sb + h * p.dq_sh;
+  float* o2 = p.dv + b * p.dv_sb + h * p.dv_sh;
   const int64_t o1_ss = kKeys ? p.dk_ss : p.dq_ss;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -371,26 +417,26 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
 #pragma unroll
     for (int c = 0; c < 4 * DC; ++c) {
       const int d = c / 4 * 64 + tx * 4 + c % 4;
-      o1[row * o1_ss + d] = static_cast<T>(acc1[i][c] * p.scale);
-      if (kKeys) o2[row * p.dv_ss + d] = static_cast<T>(acc2[i][c]);
+      o1[row * o1_ss + d] = acc1[i][c] * p.scale;
+      if (kKeys) o2[row * p.dv_ss + d] = acc2[i][c];
     }
   }
 }
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(256) bsa_bwd_simt_kernel(const SimtBwdParams p) {
   if (static_cast<int>(blockIdx.x) < p.tiles_k)
-    simt_tile<T, D, true>(p, blockIdx.y, blockIdx.x);
+    simt_tile<D, true>(p, blockIdx.y, blockIdx.x);
   else
-    simt_tile<T, D, false>(p, blockIdx.y, blockIdx.x - p.tiles_k);
+    simt_tile<D, false>(p, blockIdx.y, blockIdx.x - p.tiles_k);
 }
 
-template <typename T, int D>
+template <int D>
 int32_t launch_simt(const SimtBwdParams& p, int tiles_q, int BH, cudaStream_t st) {
   const int smem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
-  SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_bwd_simt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_bwd_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const dim3 grid(static_cast<unsigned>(p.tiles_k + tiles_q), static_cast<unsigned>(BH));
-  bsa_bwd_simt_kernel<T, D><<<grid, 256, smem, st>>>(p);
+  bsa_bwd_simt_kernel<D><<<grid, 256, smem, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
 }
@@ -480,9 +526,20 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
   pp.w = layout(q, k, block_m, block_n, static_cast<uint8_t*>(workspace));
   pp.status = device_status_ptr();
   if (pp.status == nullptr) return SAF_ERR_CUDA;
+  if (q->dtype != SAF_F32) {
+    pp.lse_factor = kLog2e;
+    pp.lse_shift = q->dtype == SAF_F16 ? bwd_f16_p_log2_scale() : 0.f;
+    pp.items = 1;
+    SAF_CUDA_TRY(cudaMemsetAsync(pp.w.class_count, 0, (kClasses + 1) * sizeof(int32_t), st));
+    rc = q->dtype == SAF_BF16 ? launch_prep<__nv_bfloat16>(pp, BH, st) : launch_prep<__half>(pp, BH, st);
+    if (rc != SAF_OK) return rc;
+    return bsa_bwd_sm100(dout, q, k, v, dq, dk, dv, block_m, block_n, sm_scale, pp.w, st);
+  }
+  if ((rc = launch_prep<float>(pp, BH, st)) != SAF_OK) return rc;
   SimtBwdParams sp{};
-  sp.q = q->data, sp.k = k->data, sp.v = v->data, sp.dout = dout->data;
-  sp.dq = dq->data, sp.dk = dk->data, sp.dv = dv->data;
+  sp.q = static_cast<const float*>(q->data), sp.k = static_cast<const float*>(k->data);
+  sp.v = static_cast<const float*>(v->data), sp.dout = static_cast<const float*>(dout->data);
+  sp.dq = static_cast<float*>(dq->data), sp.dk = static_cast<float*>(dk->data), sp.dv = static_cast<float*>(dv->data);
   sp.q_sb = q->stride_b, sp.q_sh = q->stride_h, sp.q_ss = q->stride_s;
   sp.k_sb = k->stride_b, sp.k_sh = k->stride_h, sp.k_ss = k->stride_s;
   sp.v_sb = v->stride_b, sp.v_sh = v->stride_h, sp.v_ss = v->stride_s;
@@ -495,17 +552,6 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
   sp.tiles_k = static_cast<int>((k->S + kT - 1) / kT);
   const int tiles_q = static_cast<int>((q->S + kT - 1) / kT);
   sp.scale = sm_scale;
-  sp.lse_unit = 1.f;
   sp.w = pp.w;
-  sp.merge_q = pp.merge_q, sp.merge_k = pp.merge_k;
-  if (q->dtype == SAF_F32) {
-    if ((rc = launch_prep<float>(pp, BH, st)) != SAF_OK) return rc;
-    return q->D == 64 ? launch_simt<float, 64>(sp, tiles_q, BH, st) : launch_simt<float, 128>(sp, tiles_q, BH, st);
-  }
-  if (q->dtype == SAF_BF16) {
-    if ((rc = launch_prep<__nv_bfloat16>(pp, BH, st)) != SAF_OK) return rc;
-    return launch_simt<__nv_bfloat16, 64>(sp, tiles_q, BH, st);
-  }
-  if ((rc = launch_prep<__half>(pp, BH, st)) != SAF_OK) return rc;
-  return launch_simt<__half, 64>(sp, tiles_q, BH, st);
+  return q->D == 64 ? launch_simt<64>(sp, tiles_q, BH, st) : launch_simt<128>(sp, tiles_q, BH, st);
 }

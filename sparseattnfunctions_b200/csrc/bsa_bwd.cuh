@@ -22,15 +22,25 @@ namespace saf {
 // a 128-token tile of the 16-bit kernel.  Lists: [BH, lines, cap] entries
 // block index | live halves of the line << 14, ascending; counts [BH, lines].
 struct BwdWorkspace {
-  float* stat_lse;    // [BH, Sp]: lse (log2 units for the 16-bit kernel), +inf where nothing is seen
-  float* stat_delta;  // [BH, Sp]
+  float* stat_lse;    // [BH, Sp]: -lse (16-bit kernel: in log2 units, plus p's scale), -inf where nothing is seen
+  float* stat_delta;  // [BH, Sp]: -delta
   uint16_t* list_q;   // dq lines -> key blocks
   uint16_t* list_k;   // dk / dv lines -> query blocks
   int32_t* count_q;
   int32_t* count_k;
+  // 16-bit kernel only: work items by length (longest class first) and the
+  // counters, zeroed before the preparation; the largest |do| of each 128 rows
+  uint32_t* items;       // [kClasses][BH (lines_q + lines_k)]: (1 << 31 for dk / dv) | head * lines + line
+  int32_t* class_count;  // [kClasses]
+  int32_t* next;         // the next item to take
+  float* amax;           // [BH, Sp / 128]
   int lines_q, lines_k, cap_q, cap_k;
   int64_t Sp;  // Sq rounded up to 128
   size_t bytes;
 };
+
+// Length classes of the work items: class 15 - floor(log2(blocks)), so that
+// the longest lists start first and the short ones fill the last wave.
+constexpr int kClasses = 16;
 
 }  // namespace saf
