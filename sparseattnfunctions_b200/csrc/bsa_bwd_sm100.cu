@@ -22,12 +22,13 @@
 //                next item's are there when it starts) and of the walked tiles
 //                (ring of kStages, with their lse and delta)
 //   warp 1       TMEM allocation; one thread issues S and dP of tile after
-//                tile, as soon as the one before is read out of TMEM
-//   warp 2       one thread issues the dv and dk (dq) products (one thread
-//                alone cannot issue 24 MMAs a tile fast enough)
+//                tile, as soon as the ones before are read out of TMEM
+//   warp 2       one thread issues the dv and dk (dq) products
 //   warp 3       stores finished tiles by TMA from the item's own-operand slot
-//   warps 4-19   compute: warpgroup w has columns [32 w, 32 w + 32) of a tile;
-//                four warps a sub-partition cover each other's hand-overs
+//   warps 4-19   compute: warpgroup w has columns [32 w, 32 w + 32) of a tile.
+//                A tile costs a warp two hand-overs each way: S and dP are read
+//                together (and may be overwritten at once), P and dS written
+//                together.
 // TMEM columns: S 128 | dP 128 | P 64 | dS 64 | dv 64 | dk or dq 64.
 //
 // f16: p below 2^-14 and ds of small gradients would leave the type's normal
@@ -87,7 +88,7 @@ struct Layout {
   static constexpr int kOffItem = kOffStat + kStages * kStat;
   static constexpr int kOffEnt = kOffItem + 2 * static_cast<int>(sizeof(Item));
   static constexpr int kOffBar = kOffEnt + kStages * 16;
-  static constexpr int kBars = 4 + 2 * kStages + 13;
+  static constexpr int kBars = 4 + 2 * kStages + 9;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffMisc + 16;
   static constexpr int kDynSmem = kBytes + 1024;  // slack for 1024-byte alignment
@@ -123,18 +124,14 @@ struct Ctx {
   __device__ uint32_t full(int s) const { return bar0 + 8u * (4 + s); }
   __device__ uint32_t empty(int s) const { return bar0 + 8u * (4 + kStages + s); }
   __device__ uint32_t at(int i) const { return bar0 + 8u * (4 + 2 * kStages + i); }
-  __device__ uint32_t s_full() const { return at(0); }     // S is in TMEM
-  __device__ uint32_t s_empty() const { return at(1); }    // and read
-  __device__ uint32_t dp_full() const { return at(2); }
-  __device__ uint32_t dp_empty() const { return at(3); }
-  __device__ uint32_t p_full() const { return at(4); }     // P is in TMEM
-  __device__ uint32_t p_empty() const { return at(5); }    // and multiplied
-  __device__ uint32_t ds_full() const { return at(6); }
-  __device__ uint32_t ds_empty() const { return at(7); }
-  __device__ uint32_t acc_full() const { return at(8); }   // the item's sums are final
-  __device__ uint32_t acc_empty() const { return at(9); }  // and read
-  __device__ uint32_t staged() const { return at(10); }    // the results are in shared memory
-  __device__ uint32_t drain(int w) const { return at(11 + w); }
+  __device__ uint32_t scores() const { return at(0); }     // S and dP are in TMEM
+  __device__ uint32_t read() const { return at(1); }       // and read
+  __device__ uint32_t written() const { return at(2); }    // P and dS are; the stage's values are read
+  __device__ uint32_t added() const { return at(3); }      // and multiplied
+  __device__ uint32_t acc_full() const { return at(4); }   // the item's sums are final
+  __device__ uint32_t acc_empty() const { return at(5); }  // and read
+  __device__ uint32_t staged() const { return at(6); }     // the results are in shared memory
+  __device__ uint32_t drain(int w) const { return at(7 + w); }
   __device__ bool wait(uint32_t bar, uint32_t parity) const { 
     return mbar_wait(bar, parity, abort_flag, p.status, p.budget_ns);
   }
@@ -143,6 +140,13 @@ struct Ctx {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, p.budget_ns));
   }
 };
+
+// A compute warp's wait: after a time-out it goes on (the abort flag is up, so
+// no later wait holds it, and it leaves at the end of the item).
+__device__ __forceinline__ void pass(const Ctx& c, uint32_t bar, uint32_t parity) {
+  if (!mbar_try_wait(bar, parity)) (void)c.wait(bar, parity);
+  __syncwarp();
+}
 
 __device__ __forceinline__ void warp_arrive(uint32_t bar, int lane) {
   __syncwarp();
@@ -165,97 +169,77 @@ __device__ __forceinline__ uint32_t pack2(f2 x) {
   return kBF16 ? pack_bf16x2(lo2(x), hi2(x)) : pack_f16x2(lo2(x), hi2(x));
 }
 
-// One tile: 32 columns of this thread's row.  t, tk: the tile's number in the
-// CTA and among those of dk / dv items.  kKeys: lse and delta per column
-// (shared memory), and P goes to TMEM too.  Returns false when a wait gave up.
+__device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) asm volatile("mov.b32 %0, 0;" : "=r"(r[e]));
+}
+
+// One tile: 32 columns of this thread's row; t is the tile's number in the
+// CTA.  kKeys: lse and delta per column (shared
+// memory), and P goes to TMEM too.
 template <bool kKeys, bool kBF16>
-__device__ __forceinline__ bool compute_tile(const Ctx& c, const BwdParams& p, int w, int lane, int quarter, int t,
-                                             int tk, float nl_row, float nd_row, float ds_scale) {
+__device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, int t,
+                                             float nl_row, float nd_row, float ds_scale) {
   const int s = t % kStages;
   const uint32_t par = t & 1;
-  const uint32_t tm = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  if (!c.wait_all(c.full(s), (t / kStages) & 1)) return false;
+  const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t ts = lane_addr + w * kCols;
+  const uint32_t tp = lane_addr + w * (kCols / 2);
+  pass(c, c.full(s), (t / kStages) & 1);
+  pass(c, c.scores(), par);
+  tc_fence_after();
+  uint32_t r[32], rd[32];
+  tmem_ld32(ts + kColS, r);
+  tmem_ld32(ts + kColDP, rd);
   const int2 ent = c.ents[2 * s + (w >> 1)];
-  const bool live = (ent.y >> (quarter >> 1)) & 1;
   const float4* nl = reinterpret_cast<const float4*>(c.stats + s * 2 * kM + w * kCols);
   const float4* nd = nl + kM / 4;
-  if (!c.wait_all(c.s_full(), par)) return false;
-  tc_fence_after();
-  uint32_t r[32];
-  tmem_ld32(tm + kColS + w * kCols, r);
   tmem_wait_ld(r);
+  tmem_wait_ld(rd);
   tc_fence_before();
-  warp_arrive(c.s_empty(), lane);
+  mbar_arrive(c.read());
   const f2 sl = mk2(p.scale_log2, p.scale_log2);
-  f2 pr[kCols / 2];
+  uint32_t pk[kCols / 2], dk[kCols / 2];
 #pragma unroll
   for (int e4 = 0; e4 < kCols / 4; ++e4) {
-    f2 off[2] = {mk2(nl_row, nl_row), mk2(nl_row, nl_row)};
+    f2 ol[2] = {mk2(nl_row, nl_row), mk2(nl_row, nl_row)}, od[2] = {mk2(nd_row, nd_row), mk2(nd_row, nd_row)};
     if constexpr (kKeys) {
-      const float4 l = nl[e4];
-      off[0] = mk2(l.x, l.y);
-      off[1] = mk2(l.z, l.w);
+      const float4 l = nl[e4], d = nd[e4];
+      ol[0] = mk2(l.x, l.y), ol[1] = mk2(l.z, l.w);
+      od[0] = mk2(d.x, d.y), od[1] = mk2(d.z, d.w);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int e = 4 * e4 + 2 * i;
-      const f2 y = fma2(mk2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, off[i]);
-      pr[e / 2] = mk2(ex2_approx(lo2(y)), ex2_approx(hi2(y)));
+      f2 y = fma2(mk2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, ol[i]);
+      y = mk2(ex2_approx(lo2(y)), ex2_approx(hi2(y)));
+      if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(y);
+      f2 z = add2(mk2(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]);
+      z = mul2(z, y);
+      if constexpr (!kBF16) z = mul2(z, mk2(ds_scale, ds_scale));
+      dk[e / 2] = pack2<kBF16>(z);
     }
   }
-  uint32_t pk[kCols / 2];
-  if constexpr (kKeys) {
-#pragma unroll
-    for (int e = 0; e < kCols / 2; ++e) pk[e] = live ? pack2<kBF16>(pr[e]) : 0u;
-    if (!c.wait_all(c.p_empty(), (tk & 1) ^ 1)) return false;
-    tc_fence_after();
-    tmem_st16(tm + kColP + w * (kCols / 2), pk);
-    tmem_wait_st();
-    tc_fence_before();
-    warp_arrive(c.p_full(), lane);
-  } else {
+  if (!((ent.y >> (quarter >> 1)) & 1)) {  // not listed for this half of the own tile, or no second unit
+    zero16(dk);
+    if constexpr (kKeys) zero16(pk);
+  }
+  if constexpr (!kKeys) {
     // keys past the end: their scores are 0, not -inf
     const int valid = p.Sk - (ent.x + (w & 1) * kCols);
     if (valid < kCols) {
 #pragma unroll
       for (int e = 0; e < kCols / 2; ++e)
-        pr[e] = mk2(2 * e < valid ? lo2(pr[e]) : 0.f, 2 * e + 1 < valid ? hi2(pr[e]) : 0.f);
+        dk[e] = 2 * e + 1 < valid ? dk[e] : 2 * e < valid ? dk[e] & 0xffffu : 0u;
     }
   }
-  if (!c.wait_all(c.dp_full(), par)) return false;
+  pass(c, c.added(), par ^ 1);  // the tile before is multiplied
   tc_fence_after();
-  tmem_ld32(tm + kColDP + w * kCols, r);
-  tmem_wait_ld(r);
-  tc_fence_before();
-  warp_arrive(c.dp_empty(), lane);
-#pragma unroll
-  for (int e4 = 0; e4 < kCols / 4; ++e4) {
-    f2 off[2] = {mk2(nd_row, nd_row), mk2(nd_row, nd_row)};
-    if constexpr (kKeys) {
-      const float4 d = nd[e4];
-      off[0] = mk2(d.x, d.y);
-      off[1] = mk2(d.z, d.w);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 4 * e4 + 2 * i;
-      f2 y = add2(mk2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), off[i]);
-      y = mul2(y, pr[e / 2]);
-      if constexpr (!kBF16) y = mul2(y, mk2(ds_scale, ds_scale));
-      pk[e / 2] = live ? pack2<kBF16>(y) : 0u;
-    }
-  }
-  if (!c.wait_all(c.ds_empty(), par ^ 1)) return false;
-  tc_fence_after();
-  tmem_st16(tm + kColDS + w * (kCols / 2), pk);
+  if constexpr (kKeys) tmem_st16(tp + kColP, pk);
+  tmem_st16(tp + kColDS, dk);
   tmem_wait_st();
   tc_fence_before();
-  __syncwarp();
-  if (lane == 0) {
-    mbar_arrive(c.ds_full());
-    mbar_arrive(c.empty(s));  // lse, delta and the entry are read
-  }
-  return true;
+  mbar_arrive(c.written());
 }
 
 template <bool kBF16>
@@ -284,16 +268,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(c.full(s), 1);
-      mbar_init(c.empty(s), 1 + kComputeWarps);
+      mbar_init(c.empty(s), 1);
     }
-    mbar_init(c.s_full(), 1);
-    mbar_init(c.s_empty(), kComputeWarps);
-    mbar_init(c.dp_full(), 1);
-    mbar_init(c.dp_empty(), kComputeWarps);
-    mbar_init(c.p_full(), kComputeWarps);
-    mbar_init(c.p_empty(), 1);
-    mbar_init(c.ds_full(), kComputeWarps);
-    mbar_init(c.ds_empty(), 1);
+    mbar_init(c.scores(), 1);
+    mbar_init(c.read(), 32 * kComputeWarps);
+    mbar_init(c.written(), 32 * kComputeWarps);
+    mbar_init(c.added(), 1);
     mbar_init(c.acc_full(), 1);
     mbar_init(c.acc_empty(), kComputeWarps);
     mbar_init(c.staged(), kComputeWarps);
@@ -451,16 +431,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < n; ++j, ++t) {
             const int s = t % kStages;
             const uint32_t b = walk_lo + s * (2 * L::kTile >> 4);
-            ok = c.wait(c.full(s), (t / kStages) & 1) && c.wait(c.s_empty(), (t & 1) ^ 1);
+            ok = c.wait(c.full(s), (t / kStages) & 1) && c.wait(c.read(), (t & 1) ^ 1);
             if (!ok) break;
             tc_fence_after();
             scores(kColS, a, b);
-            tc_commit(c.s_full());
-            ok = c.wait(c.dp_empty(), (t & 1) ^ 1);
-            if (!ok) break;
-            tc_fence_after();
             scores(kColDP, a + (L::kTile >> 4), b + (L::kTile >> 4));
-            tc_commit(c.dp_full());
+            tc_commit(c.scores());
           }
           if (n > 0)
             tc_commit(c.own_empty(slot));
@@ -487,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc_mma_ts(c.tmem + d, c.tmem + a + kk * 8, desc64(b + kk * 128), kIdesc, 1u);
           }
         };
-        int it = 0, t = 0, tk = 0, na = 0;  // na: items with tiles
+        int it = 0, t = 0, na = 0;  // na: items with tiles
         bool ok = true;
         while (ok) {
           const int slot = it & 1;
@@ -503,20 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < n; ++j, ++t) {
             const int s = t % kStages;
             const uint32_t b = walk_lo + s * (2 * L::kTile >> 4);
-            ok = c.wait(keys ? c.p_full() : c.ds_full(), keys ? (tk & 1) : (t & 1));
+            ok = c.wait(c.written(), t & 1);
             if (!ok) break;
             tc_fence_after();
             const bool both = c.ents[2 * s + 1].y != 0;
-            if (keys) {
-              add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
-              tc_commit(c.p_empty());
-              ++tk;
-              ok = c.wait(c.ds_full(), t & 1);
-              if (!ok) break;
-              tc_fence_after();
-            }
+            if (keys) add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
             add(kColK, kColDS, b, both, j > 0);
-            tc_commit(c.ds_empty());
+            tc_commit(c.added());
             tc_commit(c.empty(s));
           }
           if (ok && n > 0) tc_commit(c.acc_full());
@@ -559,24 +528,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = (warp >> 2) - 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    int it = 0, t = 0, tk = 0, na = 0;
+    int it = 0, t = 0, na = 0;
     while (true) {
       const int slot = it & 1;
       if (!c.wait_all(c.own_full(slot), (it >> 1) & 1)) break;
       const int keys = c.items[slot].keys, n = c.items[slot].n;
       if (keys < 0) break;
       const float ds_scale = kBF16 ? 1.f : c.items[slot].ds_scale;
-      bool ok = true;
       if (keys) {
-        for (int j = 0; j < n && ok; ++j, ++t, ++tk)
-          ok = compute_tile<true, kBF16>(c, p, w, lane, quarter, t, tk, 0.f, 0.f, ds_scale);
+        for (int j = 0; j < n; ++j, ++t) compute_tile<true, kBF16>(c, p, w, quarter, t, 0.f, 0.f, ds_scale);
       } else {
         const int64_t at = c.items[slot].g * p.w.Sp + c.items[slot].tile * kM + row;
         const float nl = p.w.stat_lse[at], nd = p.w.stat_delta[at];
-        for (int j = 0; j < n && ok; ++j, ++t)
-          ok = compute_tile<false, kBF16>(c, p, w, lane, quarter, t, tk, nl, nd, ds_scale);
+        for (int j = 0; j < n; ++j, ++t) compute_tile<false, kBF16>(c, p, w, quarter, t, nl, nd, ds_scale);
       }
-      if (!ok) break;
+      if (__any_sync(0xffffffffu, *c.abort_flag)) break;
       // Results: warpgroups 0 and 1 take dv, 2 and 3 dk (32 channels each);
       // dq 16 channels each.  They go through this item's own-operand slot,
       // which no product reads once the sums are final.
