@@ -164,9 +164,26 @@ __device__ __forceinline__ uint64_t desc64(uint32_t lo) {
   return d;
 }
 
+// Register pairs by mov.b64, which costs nothing when they lie side by side.
+__device__ __forceinline__ f2 pair(float lo, float hi) {
+  f2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d.v) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float first(f2 x) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x.v));
+  return lo;
+}
+__device__ __forceinline__ float second(f2 x) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x.v));
+  return hi;
+}
+
 template <bool kBF16>
 __device__ __forceinline__ uint32_t pack2(f2 x) {
-  return kBF16 ? pack_bf16x2(lo2(x), hi2(x)) : pack_f16x2(lo2(x), hi2(x));
+  return kBF16 ? pack_bf16x2(first(x), second(x)) : pack_f16x2(first(x), second(x));
 }
 
 __device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
@@ -176,16 +193,15 @@ __device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
 
 // One tile: 32 columns of this thread's row; t is the tile's number in the
 // CTA.  kKeys: lse and delta per column (shared
-// memory), and P goes to TMEM too.
+// memory; the MMA thread that arrives on `scores` has waited for the stage),
+// and P goes to TMEM too.
 template <bool kKeys, bool kBF16>
-__device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, int t,
+__device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, uint32_t t,
                                              float nl_row, float nd_row, float ds_scale) {
-  const int s = t % kStages;
-  const uint32_t par = t & 1;
+  const uint32_t s = t % kStages, par = t & 1;
   const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t ts = lane_addr + w * kCols;
   const uint32_t tp = lane_addr + w * (kCols / 2);
-  pass(c, c.full(s), (t / kStages) & 1);
   pass(c, c.scores(), par);
   tc_fence_after();
   uint32_t r[32], rd[32];
@@ -205,17 +221,16 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
     f2 ol[2] = {mk2(nl_row, nl_row), mk2(nl_row, nl_row)}, od[2] = {mk2(nd_row, nd_row), mk2(nd_row, nd_row)};
     if constexpr (kKeys) {
       const float4 l = nl[e4], d = nd[e4];
-      ol[0] = mk2(l.x, l.y), ol[1] = mk2(l.z, l.w);
-      od[0] = mk2(d.x, d.y), od[1] = mk2(d.z, d.w);
+      ol[0] = pair(l.x, l.y), ol[1] = pair(l.z, l.w);
+      od[0] = pair(d.x, d.y), od[1] = pair(d.z, d.w);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int e = 4 * e4 + 2 * i;
-      f2 y = fma2(mk2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, ol[i]);
-      y = mk2(ex2_approx(lo2(y)), ex2_approx(hi2(y)));
-      if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(y);
-      f2 z = add2(mk2(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]);
-      z = mul2(z, y);
+      const f2 y = fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, ol[i]);
+      const f2 pr = pair(ex2_approx(first(y)), ex2_approx(second(y)));
+      if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(pr);
+      f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
       if constexpr (!kBF16) z = mul2(z, mk2(ds_scale, ds_scale));
       dk[e / 2] = pack2<kBF16>(z);
     }
@@ -263,14 +278,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(c.own_full(s), 1);
-      mbar_init(c.own_empty(s), 1 + 1 + kComputeWarps);  // score thread, store warp, compute warps
+      mbar_init(c.own_empty(s), 3 + kComputeWarps);  // MMA threads, store warp, compute warps
       mbar_init(c.drain(s), 1);
     }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(c.full(s), 1);
       mbar_init(c.empty(s), 1);
     }
-    mbar_init(c.scores(), 1);
+    mbar_init(c.scores(), 2);
     mbar_init(c.read(), 32 * kComputeWarps);
     mbar_init(c.written(), 32 * kComputeWarps);
     mbar_init(c.added(), 1);
@@ -419,17 +434,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int kk = 0; kk < kD / 16; ++kk)
             tc_mma_ss(c.tmem + d, desc64(a + kk * 2), desc64(b + kk * 2), kIdesc, kk > 0 ? 1u : 0u);
         };
-        int it = 0, t = 0;
+        uint32_t it = 0, t = 0;
         bool ok = true;
         while (ok) {
-          const int slot = it & 1;
+          const uint32_t slot = it & 1;
           if (!c.wait(c.own_full(slot), (it >> 1) & 1)) break;
           ++it;
           const int keys = c.items[slot].keys, n = c.items[slot].n;
           if (keys < 0) break;
           const uint32_t a = own_lo + slot * (2 * L::kTile >> 4);
           for (int j = 0; j < n; ++j, ++t) {
-            const int s = t % kStages;
+            const uint32_t s = t % kStages;
             const uint32_t b = walk_lo + s * (2 * L::kTile >> 4);
             ok = c.wait(c.full(s), (t / kStages) & 1) && c.wait(c.read(), (t & 1) ^ 1);
             if (!ok) break;
@@ -437,6 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(kColS, a, b);
             scores(kColDP, a + (L::kTile >> 4), b + (L::kTile >> 4));
             tc_commit(c.scores());
+            mbar_arrive(c.scores());  // hands on the order behind this thread's wait for the stage
           }
           if (n > 0)
             tc_commit(c.own_empty(slot));
@@ -463,21 +479,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc_mma_ts(c.tmem + d, c.tmem + a + kk * 8, desc64(b + kk * 128), kIdesc, 1u);
           }
         };
-        int it = 0, t = 0, na = 0;  // na: items with tiles
+        uint32_t it = 0, t = 0, na = 0;  // na: items with tiles
         bool ok = true;
         while (ok) {
-          const int slot = it & 1;
+          const uint32_t slot = it & 1;
           if (!c.wait(c.own_full(slot), (it >> 1) & 1)) break;
           ++it;
           const int keys = c.items[slot].keys, n = c.items[slot].n;
           if (keys < 0) break;
+          mbar_arrive(c.own_empty(slot));  // the entry is read
           if (n > 0) {
             ok = c.wait(c.acc_empty(), (na & 1) ^ 1);  // the sums of the item before are read
             if (!ok) break;
             ++na;
           }
           for (int j = 0; j < n; ++j, ++t) {
-            const int s = t % kStages;
+            const uint32_t s = t % kStages;
             const uint32_t b = walk_lo + s * (2 * L::kTile >> 4);
             ok = c.wait(c.written(), t & 1);
             if (!ok) break;
@@ -528,9 +545,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = (warp >> 2) - 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    int it = 0, t = 0, na = 0;
+    uint32_t it = 0, t = 0, na = 0;
     while (true) {
-      const int slot = it & 1;
+      const uint32_t slot = it & 1;
       if (!c.wait_all(c.own_full(slot), (it >> 1) & 1)) break;
       const int keys = c.items[slot].keys, n = c.items[slot].n;
       if (keys < 0) break;
@@ -570,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           x[i] = pack2<kBF16>(
-              mk2(__uint_as_float(r[8 * i8 + 2 * i]) * scale, __uint_as_float(r[8 * i8 + 2 * i + 1]) * scale));
+              pair(__uint_as_float(r[8 * i8 + 2 * i]) * scale, __uint_as_float(r[8 * i8 + 2 * i + 1]) * scale));
         // dq: the two warpgroups that read the same 32 channels store 16 each
         if (keys || (i8 >> 1) == (w & 1)) st_shared_v4(dst + (((chunk0 + i8) ^ (row & 7)) << 4), x[0], x[1], x[2], x[3]);
       }
