@@ -206,7 +206,8 @@ int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor
  * rows of split lead tiles, so launches may overlap on a device.
  * No counterpart in the reference, whose kernel has no training path
  * (utils/block_sparse_attn_kernel.py:278-281). */
-size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, int32_t block_m, int32_t lead_rows);
+size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
+                                       int32_t lead_rows);
 int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                         const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                         int64_t col_capacity, int32_t block_m, int32_t block_n, float sm_scale,

@@ -119,12 +119,13 @@ SIGNATURES = {
                            _P]),
     "saf_bsa_fwd_ranges": (_I32, [_PT4, _PT4, _PT4, _PT4, _P, _P, _I64, _I32, _I32, _P, _I64, _F32,
                                   _I32, _P, _P]),
-    "saf_bsa_fwd_lse_workspace_bytes": (_SZ, [_PT4, _I32, _I32]),
-    "saf_bsa_fwd_lse": (_I32, [_PT4, _PT4, _PT4, _PT4, _P, _P, _I64, _I32, _I32, _F32, _I32, _P, _P, _SZ, _P]),
-    "saf_bsa_bwd_workspace_bytes": (_SZ, [_PT4, _PT4, _I32, _I32]),
-    "saf_bsa_bwd": (_I32, [_PT4, _PT4, _PT4, _PT4, _PT4, _P, _I64, _PT4, _PT4, _PT4, _P, _P, _I64, _I32, _I32,
+    # (saf_tensor4 arguments of the next five as void*: kernels.py passes packed bytes)
+    "saf_bsa_fwd_lse_workspace_bytes": (_SZ, [_P, _P, _I32, _I32]),
+    "saf_bsa_fwd_lse": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _F32, _I32, _P, _P, _SZ, _P]),
+    "saf_bsa_bwd_workspace_bytes": (_SZ, [_P, _P, _I32, _I32]),
+    "saf_bsa_bwd": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I32, _I32,
                            _F32, _P, _SZ, _P]),
-    "saf_rope": (_I32, [_PT4, _PT4, _PT4, _PT4, _P, _P, _I64, _I64, _I32, _I32, _I32, _P]),
+    "saf_rope": (_I32, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P]),
     "saf_frame_mask_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
     "saf_frame_mask": (_I32, [_PT4, _PT4, _P, _I32, _I32, _I32, _I32, _F32, ctypes.c_double, _P, _SZ, _P,
                               _P, _P, _P]),

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(256) bsa_bwd_simt_kernel(const SimtBwdParams p
 template <int D>
 int32_t launch_simt(const SimtBwdParams& p, int tiles_q, int BH, cudaStream_t st) {
   const int smem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
-  SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_bwd_simt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (const int32_t rc = allow_smem<bsa_bwd_simt_kernel<D>>(smem); rc != SAF_OK) return rc;
   const dim3 grid(static_cast<unsigned>(p.tiles_k + tiles_q), static_cast<unsigned>(BH));
   bsa_bwd_simt_kernel<D><<<grid, 256, smem, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());
@@ -446,7 +446,8 @@ int32_t launch_prep(const PrepParams& p, int BH, cudaStream_t st) {
   const int words = ((p.nbq > p.nbk ? p.nbq : p.nbk) + 31) / 32;
   const int rows = p.nbq > kGroup ? p.nbq : kGroup;
   const int smem = (kGroup * words + rows + 1) * 4;
-  SAF_CUDA_TRY(cudaFuncSetAttribute(bwd_prep_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 48 * 1024)
+    if (const int32_t rc = allow_smem<bwd_prep_kernel<T>>(smem); rc != SAF_OK) return rc;
   const dim3 grid(static_cast<unsigned>(p.groups_k + p.groups_q + p.w.Sp / kRowChunk), static_cast<unsigned>(BH));
   bwd_prep_kernel<T><<<grid, 256, smem, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());

@@ -73,9 +73,9 @@ struct BwdParams {
   uint64_t budget_ns;
 };
 
-// Maps: o* tiles of 128 rows (own operands), w* walked units of 64 rows; results.
+// Tensor maps, boxes of 64 rows.
 struct Maps {
-  CUtensorMap oq, odo, ok, ov, wq, wdo, wk, wv, dq, dk, dv;
+  CUtensorMap q, dout, k, v, dq, dk, dv;
 };
 
 // Shared memory: own operands [2 slots][2][128 x 64], the ring [kStages][2]
@@ -99,7 +99,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
-// 128 x 64 tile of shared memory -> rows [row, row + 128) of one head; rows past the end are not written.
+// 64 x 64 tile of shared memory -> rows [row, row + 64) of one head; rows past the end are not written.
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int row, int h, int b) {
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -363,8 +363,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (im.n > 0) {
             mbar_arrive_expect_tx(c.own_full(slot), 2 * L::kTile);
             const uint32_t dst = c.own + slot * 2 * L::kTile;
-            tma_load_4d(dst, im.keys ? &maps.ok : &maps.oq, c.own_full(slot), 0, im.tile * kM, h, b);
-            tma_load_4d(dst + L::kTile, im.keys ? &maps.ov : &maps.odo, c.own_full(slot), 0, im.tile * kM, h, b);
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t at = dst + x * (L::kTile / 2);
+              const int r = im.tile * kM + x * kUnit;
+              tma_load_4d(at, im.keys ? &maps.k : &maps.q, c.own_full(slot), 0, r, h, b);
+              tma_load_4d(at + L::kTile, im.keys ? &maps.v : &maps.dout, c.own_full(slot), 0, r, h, b);
+            }
           } else {
             mbar_arrive(c.own_full(slot));
           }
@@ -397,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int x = 0; x < units; ++x) {
               const int row = x ? row1 : row0;
               const uint32_t dst = c.walk + s * 2 * L::kTile + x * (L::kTile / 2);
-              tma_load_4d(dst, im.keys ? &maps.wq : &maps.wk, c.full(s), 0, row, h, b);
-              tma_load_4d(dst + L::kTile, im.keys ? &maps.wdo : &maps.wv, c.full(s), 0, row, h, b);
+              tma_load_4d(dst, im.keys ? &maps.q : &maps.k, c.full(s), 0, row, h, b);
+              tma_load_4d(dst + L::kTile, im.keys ? &maps.dout : &maps.v, c.full(s), 0, row, h, b);
               if (im.keys) {
                 const int64_t at = im.g * p.w.Sp + row;
                 const uint32_t st = c.stat + s * L::kStat + x * kUnit * 4;
@@ -522,8 +526,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           const int h = im.g % p.H, b = im.g / p.H;
           const uint32_t src = c.own + slot * 2 * L::kTile;
-          tma_store_4d(im.keys ? &maps.dv : &maps.dq, src, im.tile * kM, h, b);
-          if (im.keys) tma_store_4d(&maps.dk, src + L::kTile, im.tile * kM, h, b);
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t at = src + x * (L::kTile / 2);
+            const int r = im.tile * kM + x * kUnit;
+            if (r >= (im.keys ? p.Sk : p.Sq)) break;
+            tma_store_4d(im.keys ? &maps.dv : &maps.dq, at, r, h, b);
+            if (im.keys) tma_store_4d(&maps.dk, at + L::kTile, r, h, b);
+          }
           bulk_commit();
           bulk_wait_read();
         }
@@ -613,7 +622,7 @@ int32_t launch(const Maps& maps, const BwdParams& p, int grid, cudaStream_t stre
     return cudaFuncGetAttributes(&fa, bsa_bwd_sm100_kernel<kBF16>) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (launch_regs < kLaunchRegs) return SAF_ERR_UNSUPPORTED;
-  SAF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout::kDynSmem));
+  if (const int32_t rc = allow_smem<bsa_bwd_sm100_kernel<kBF16>>(Layout::kDynSmem); rc != SAF_OK) return rc;
   kern<<<grid, kThreads, Layout::kDynSmem, stream>>>(maps, p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
@@ -632,12 +641,9 @@ int32_t bsa_bwd_sm100(const saf_tensor4* dout, const saf_tensor4* q, const saf_t
   const struct {
     CUtensorMap* map;
     const saf_tensor4* t;
-    int rows;
-  } want[11] = {{&maps.oq, q, kM},    {&maps.odo, dout, kM}, {&maps.ok, k, kM},  {&maps.ov, v, kM},
-                {&maps.wq, q, kUnit}, {&maps.wdo, dout, kUnit}, {&maps.wk, k, kUnit}, {&maps.wv, v, kUnit},
-                {&maps.dq, dq, kM},   {&maps.dk, dk, kM},    {&maps.dv, dv, kM}};
+  } want[7] = {{&maps.q, q}, {&maps.dout, dout}, {&maps.k, k}, {&maps.v, v}, {&maps.dq, dq}, {&maps.dk, dk}, {&maps.dv, dv}};
   for (const auto& x : want) {
-    const int32_t rc = make_qkv_map(x.map, x.t, x.rows);
+    const int32_t rc = make_qkv_map(x.map, x.t, kUnit);
     if (rc != SAF_OK) return rc;
   }
   BwdParams p{};
@@ -650,9 +656,8 @@ int32_t bsa_bwd_sm100(const saf_tensor4* dout, const saf_tensor4* q, const saf_t
   p.status = device_status_ptr();
   p.budget_ns = wait_budget_ns();
   if (p.status == nullptr) return SAF_ERR_CUDA;
-  int dev = 0, sms = 0;
-  SAF_CUDA_TRY(cudaGetDevice(&dev));
-  SAF_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int sms = current_device_sms();
+  if (sms <= 0) return SAF_ERR_CUDA;
   const int64_t items = static_cast<int64_t>(p.BH) * (w.lines_q + w.lines_k);
   const int grid = static_cast<int>(items < sms ? items : sms);
   return q->dtype == SAF_BF16 ? launch<true>(maps, p, grid, stream) : launch<false>(maps, p, grid, stream);

@@ -18,7 +18,7 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
                       int64_t bias_stride, float sm_scale, int lead_tiles, const int32_t* row_ranges,
                       const FrameMaskArgs* frames, const PoolArgs* pool, const TrainArgs* train,
                       cudaStream_t stream);
-int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t lead_tiles, int64_t* part_bytes);
+int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles, int64_t* part_bytes);
 int32_t bsa_fwd_sm100_keys(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                            const saf_tensor4* o, const int32_t* key_list, int32_t key_len,
                            const int32_t* key_batch, float sm_scale, cudaStream_t stream);
@@ -243,13 +243,11 @@ int32_t bsa_fwd_simt(const saf_tensor4* q, const saf_tensor4* k, const saf_tenso
   dim3 grid(static_cast<unsigned>((q->S + kT - 1) / kT), static_cast<unsigned>(q->B * q->H));
   if (q->D == 64) {
     const int smem = (3 * 64 * kT + kT * (kT + 1) + 2 * kT) * 4;
-    SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_fwd_simt_kernel<64>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (const int32_t rc = allow_smem<bsa_fwd_simt_kernel<64>>(smem); rc != SAF_OK) return rc;
     bsa_fwd_simt_kernel<64><<<grid, 256, smem, stream>>>(p);
   } else {
     const int smem = (3 * 128 * kT + kT * (kT + 1) + 2 * kT) * 4;
-    SAF_CUDA_TRY(cudaFuncSetAttribute(bsa_fwd_simt_kernel<128>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (const int32_t rc = allow_smem<bsa_fwd_simt_kernel<128>>(smem); rc != SAF_OK) return rc;
     bsa_fwd_simt_kernel<128><<<grid, 256, smem, stream>>>(p);
   }
   SAF_CUDA_TRY(cudaGetLastError());
@@ -364,10 +362,11 @@ static int64_t lead_tiles_of(int32_t lead_rows, int32_t block_m) {
   return (static_cast<int64_t>(lead_rows) * block_m + 127) / 128;
 }
 
-extern "C" size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, int32_t block_m, int32_t lead_rows) {
-  if (check_tensor4(q) != SAF_OK || block_m <= 0 || lead_rows < 0 || q->dtype == SAF_F32) return 0;
+extern "C" size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
+                                                 int32_t lead_rows) {
+  if (check_tensor4(q) != SAF_OK || check_tensor4(k) != SAF_OK || block_m <= 0 || lead_rows < 0 || q->dtype == SAF_F32) return 0;
   int64_t part;
-  return static_cast<size_t>(bsa_train_split_bytes(q->B * q->H, q->S, lead_tiles_of(lead_rows, block_m), &part));
+  return static_cast<size_t>(bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), &part));
 }
 
 extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
@@ -383,10 +382,8 @@ extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, c
     if ((rc = check_operand(t, q)) != SAF_OK) return rc;
   TrainArgs train{lse, nullptr, nullptr};
   if (q->dtype != SAF_F32) {
-    DeviceScope dev_scope;
-    if ((rc = dev_scope.bind(q->data)) != SAF_OK) return rc;
     int64_t part = 0;
-    const int64_t need = bsa_train_split_bytes(q->B * q->H, q->S, lead_tiles_of(lead_rows, block_m), &part);
+    const int64_t need = bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), &part);
     if (need > 0) {
       if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) return SAF_ERR_WORKSPACE;
       if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;

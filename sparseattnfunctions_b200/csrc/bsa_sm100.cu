@@ -1221,11 +1221,20 @@ int32_t split_buffers(float** part, int** cnt) {
   return SAF_OK;
 }
 
+// SMs that the training forward's split is sized for (its workspace must not
+// depend on the device that the bytes were asked on).
+constexpr int kTrainSms = 148;
+
 // The most work items one lead tile may be cut into: enough to fill the
 // GPU's CTAs, at most 8.
 int split_cap(int64_t items, int sms) {
   return static_cast<int>(std::min<int64_t>(8, (2 * sms + items - 1) / items));
 }
+
+// The training forward splits lead tiles of 25 blocks of 128 keys or more:
+// at two heads, 20 blocks take 31.6 us unsplit and 32.8 split (the counters'
+// clearing and the merge), 33 blocks 47.2 and 35.0, 139 blocks 181 and 60.
+int train_split_cap(int64_t items, int64_t Sk) { return Sk > 24 * 128 ? split_cap(items, kTrainSms) : 1; }
 
 template <int BN, bool kBias, bool kBF16, int kMask>
 int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
@@ -1233,7 +1242,8 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   auto kern = bsa_fwd_sm100_kernel<BN, kBias, kBF16, kMask>;
   p.list_cap = (p.nbk + 7) / 8 * 8;
   const int smem = Layout<BN, kBias>::kDynSmem + list_smem_bytes(p.list_cap, p.nbk);
-  SAF_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  int32_t rc = allow_smem<bsa_fwd_sm100_kernel<BN, kBias, kBF16, kMask>>(smem);
+  if (rc != SAF_OK) return rc;
   // setmaxnreg.inc only draws on the registers the CTA was launched with: a
   // build that launched with fewer than the split needs would wait forever
   static const int launch_regs = [] {
@@ -1242,11 +1252,9 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
                                                                                                   : 0;
   }();
   if (launch_regs * kThreads < 128 * static_cast<int>(kRegsCtl + kRegsSoftmax)) return SAF_ERR_UNSUPPORTED;
-  int dev = 0, sms = 0;
-  SAF_CUDA_TRY(cudaGetDevice(&dev));
-  SAF_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  int32_t rc = tile_counter_slot(&p.tile_ctr);
-  if (rc != SAF_OK) return rc;
+  const int sms = current_device_sms();
+  if (sms <= 0) return SAF_ERR_CUDA;
+  if ((rc = tile_counter_slot(&p.tile_ctr)) != SAF_OK) return rc;
   p.n_tiles = n_tiles;
   p.BH = p.B * p.H;
   // Lead tiles (dense text rows: every key block) are the longest work items;
@@ -1258,7 +1266,7 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   p.splits = 1;
   if (lead > 0 && kMask != kMaskPool && kMask != kMaskKeys) {
     const int64_t items = static_cast<int64_t>(lead) * p.BH;
-    int sp = split_cap(items, sms);
+    const int sp = kMask == kMaskTrain ? train_split_cap(items, p.Sk) : split_cap(items, sms);
     // the training forward brings its own buffers, so that its launches may
     // overlap (the host entry sized them by the same rule)
     if (kMask == kMaskTrain) {
@@ -1283,13 +1291,9 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
 
 // Bytes of the split buffers of a training forward (0: its lead tiles run
 // unsplit): partial rows, then one counter per lead row.
-int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t lead_tiles, int64_t* part_bytes) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
-    sms = 256;  // no device here: an upper bound for any sm_100 part
+int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles, int64_t* part_bytes) {
   const int64_t items = std::min<int64_t>(lead_tiles, (Sq + kBM - 1) / kBM) * BH;
-  const int sp = items > 0 ? split_cap(items, sms) : 1;
+  const int sp = items > 0 ? train_split_cap(items, Sk) : 1;
   *part_bytes = sp > 1 ? items * sp * kBM * kSplitRow * static_cast<int64_t>(sizeof(float)) : 0;
   return sp > 1 ? *part_bytes + items * kBM * static_cast<int64_t>(sizeof(int)) : 0;
 }

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/saf_api.h"
 
 #define SAF_CUDA_TRY(expr)                               \
@@ -36,6 +38,8 @@ CUresult encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, cuuint32
 int32_t make_qkv_map(CUtensorMap* map, const saf_tensor4* t, int rows);
 // Current device is sm_100 (B200 family).
 bool current_device_is_sm100();
+// Its SM count (0 when it cannot be read).
+int current_device_sms();
 // Makes the device that owns a pointer current for one entry point and puts
 // the calling thread's previous current device back when the scope ends, so
 // a C caller's later runtime calls land on the device it had selected.
@@ -50,6 +54,22 @@ class DeviceScope {
  private:
   int prev_ = -1;  // device to restore, or -1 when nothing was changed
 };
+
+// Raises a kernel's dynamic shared memory limit on the current device to
+// `bytes` where it is not there yet (the attribute call costs about a
+// microsecond a launch).
+template <auto kKernel>
+int32_t allow_smem(int bytes) {
+  static std::atomic<int> allowed[64] = {};
+  int dev = 0;
+  SAF_CUDA_TRY(cudaGetDevice(&dev));
+  const bool known = dev >= 0 && dev < 64;
+  if (!known || allowed[dev].load(std::memory_order_relaxed) < bytes) {
+    SAF_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (known) allowed[dev].store(bytes, std::memory_order_relaxed);
+  }
+  return SAF_OK;
+}
 
 inline int elem_bytes(int32_t dtype) { return dtype == SAF_F32 ? 4 : 2; }
 

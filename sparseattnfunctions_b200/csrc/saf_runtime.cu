@@ -84,15 +84,37 @@ int32_t make_qkv_map(CUtensorMap* map, const saf_tensor4* t, int rows) {
   return r == CUDA_SUCCESS ? SAF_OK : SAF_ERR_STRIDE;
 }
 
-bool current_device_is_sm100() {
+namespace {
+// Compute capability (10 * major + minor) and SM count of the current device,
+// read from the driver once per device.
+bool device_facts(int* cc, int* sms) {
+  static std::atomic<int> known[kMaxDevices] = {};  // cc << 16 | sms
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  int major = 0, minor = 0;
-  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-    return false;
-  if (cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess)
-    return false;
-  return major == 10 && minor == 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+  int v = known[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    int major = 0, minor = 0, n = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return false;
+    v = (10 * major + minor) << 16 | n;
+    known[dev].store(v, std::memory_order_relaxed);
+  }
+  *cc = v >> 16;
+  *sms = v & 0xffff;
+  return true;
+}
+}  // namespace
+
+bool current_device_is_sm100() {
+  int cc = 0, sms = 0;
+  return device_facts(&cc, &sms) && cc == 100;
+}
+
+int current_device_sms() {
+  int cc = 0, sms = 0;
+  return device_facts(&cc, &sms) ? sms : 0;
 }
 
 int32_t DeviceScope::bind(const void* ptr) {

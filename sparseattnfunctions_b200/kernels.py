@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -35,8 +36,19 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-def _stream_ptr(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _stream_ptr(dev) -> int:
+    """cudaStream_t of the current stream of ``dev`` (a device or its index),
+    without building the stream object (0.1 against 2.3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev if isinstance(dev, int) else dev.index)
+
+
+def _device_of(*tensors: torch.Tensor) -> int:
+    """Index of the one CUDA device that all ``tensors`` are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            _require_cuda(*tensors)
+    return index
 
 
 def _t4(x: torch.Tensor) -> _lib.Tensor4:
@@ -46,12 +58,18 @@ def _t4(x: torch.Tensor) -> _lib.Tensor4:
         raise ValueError(f"unsupported dtype {x.dtype}")
     if x.stride(-1) != 1:
         raise ValueError("the last (D) dimension must be contiguous")
-    t = _lib.Tensor4()
-    t.data = x.data_ptr()
-    t.dtype = _DTYPES[x.dtype]
-    t.B, t.H, t.S, t.D = x.shape
-    t.stride_b, t.stride_h, t.stride_s = x.stride(0), x.stride(1), x.stride(2)
-    return t
+    B, H, S, D = x.shape
+    sb, sh, ss, _ = x.stride()
+    return _lib.Tensor4(x.data_ptr(), _DTYPES[x.dtype], 0, B, H, S, D, sb, sh, ss)
+
+
+_PACK_T4 = struct.Struct("Pii7q").pack  # saf_tensor4
+
+
+def _p4(x: torch.Tensor) -> bytes:
+    """saf_tensor4 of a [B, H, S, D] tensor with a contiguous D, packed (half
+    the cost of a ctypes structure; ctypes passes the bytes by address)."""
+    return _PACK_T4(x.data_ptr(), _DTYPES[x.dtype], 0, *x.shape, *x.stride()[:3])
 
 
 def _d_last(x: torch.Tensor) -> torch.Tensor:
@@ -388,6 +406,12 @@ def bsa_fwd_pool(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCS
     return out, pool
 
 
+def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[:2] != qs[:2] or ks[3] != qs[3]:
+        raise ValueError(f"q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} do not match")
+
+
 def _check_csr(csr: BlockCSR, q: torch.Tensor, k: torch.Tensor) -> None:
     B, H, Sq, _ = q.shape
     if (csr.B, csr.H) != (B, H) or csr.nbq != math.ceil(Sq / csr.block_m) or \
@@ -416,33 +440,30 @@ def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR
     ``csr`` and the row log-sum-exp that ``bsa_bwd`` needs.  Returns ``(out,
     lse)``, ``lse`` fp32 ``[B, H, Sq]`` in natural units; a row with no live
     key gives zeros and ``-inf`` (``bsa_fwd`` gives NaN there)."""
-    dev = _require_cuda(q, k, v, csr.row_ptr, csr.col_idx)
+    dev = _device_of(q, k, v, csr.row_ptr, csr.col_idx)
     q, k, v = _d_last(q), _d_last(k), _d_last(v)
-    if q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or v.shape != k.shape or \
-            k.shape[3] != q.shape[3]:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
-    B, H, Sq, D = q.shape
+    _check_qkv(q, k, v)
     _check_csr(csr, q, k)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have the shape, type and device of q")
-    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
     if q.numel() == 0 or k.numel() == 0:  # no key at all is a row without a live key
         return out.zero_(), lse.fill_(-math.inf)
     lib = _lib.load()
-    tq, tk, tv, to = _t4(q), _t4(k), _t4(v), _t4(out)
-    lead = int(csr.dense_rows)
-    ws, ws_bytes = None, 0
+    tq, tk, tv, to = _p4(q), _p4(k), _p4(v), _p4(out)
+    lead, ws_bytes, ws_ptr = int(csr.dense_rows), 0, None
     if lead > 0:
-        with torch.cuda.device(dev):
-            ws_bytes = int(lib.saf_bsa_fwd_lse_workspace_bytes(ctypes.byref(tq), csr.block_m, lead))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = lib.saf_bsa_fwd_lse(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(to),
-                             csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
-                             csr.block_n, float(sm_scale), lead, lse.data_ptr(),
-                             ws.data_ptr() if ws_bytes else None, ws_bytes, _stream_ptr(dev))
-    _lib.check("saf_bsa_fwd_lse", rc)
+        ws_bytes = lib.saf_bsa_fwd_lse_workspace_bytes(tq, tk, csr.block_m, lead)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            ws_ptr = ws.data_ptr()
+    rc = lib.saf_bsa_fwd_lse(tq, tk, tv, to, csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(),
+                             csr.block_m, csr.block_n, sm_scale, lead, lse.data_ptr(), ws_ptr, ws_bytes,
+                             _stream_ptr(dev))
+    if rc:
+        _lib.check("saf_bsa_fwd_lse", rc)
     return out, lse
 
 
@@ -453,31 +474,31 @@ def bsa_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     returned.  The probabilities are recomputed block by block; rows and keys
     that no block lists get zeros.  Equal inputs give equal bits
     (saf_bsa_bwd)."""
-    dev = _require_cuda(dout, q, k, v, out, lse, csr.row_ptr, csr.col_idx)
+    dev = _device_of(dout, q, k, v, out, lse, csr.row_ptr, csr.col_idx)
     dout = _rows_last(dout, 1 if dout.dtype == torch.float32 else 8)
     q, k, v, out = _d_last(q), _d_last(k), _d_last(v), _d_last(out)
-    if dout.dim() != 4 or q.dim() != 4 or k.dim() != 4 or k.shape[:2] != q.shape[:2] or v.shape != k.shape or \
-            k.shape[3] != q.shape[3] or dout.shape != q.shape or out.shape != q.shape:
-        raise ValueError(f"dout {tuple(dout.shape)}, q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, "
-                         f"out {tuple(out.shape)} do not match")
+    _check_qkv(q, k, v)
     _check_csr(csr, q, k)
+    if dout.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"dout {tuple(dout.shape)} and out {tuple(out.shape)} must match q {tuple(q.shape)}")
     if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
         raise ValueError(f"lse must be a float32 {list(q.shape[:3])} tensor")
-    if lse.stride(2) != 1 or lse.stride(1) < lse.shape[2] or lse.stride(0) != lse.shape[1] * lse.stride(1):
+    lb, lh, ls = lse.stride()
+    if ls != 1 or lh < lse.shape[2] or lb != lse.shape[1] * lh:
         lse = lse.contiguous()
+        lh = lse.stride(1)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     lib = _lib.load()
-    tq, tk = _t4(q), _t4(k)
-    ts = [_t4(x) for x in (dout, v, out, dq, dk, dv)]
-    tdo, tv, to, tdq, tdk, tdv = (ctypes.byref(t) for t in ts)
-    ws_bytes = int(lib.saf_bsa_bwd_workspace_bytes(ctypes.byref(tq), ctypes.byref(tk), csr.block_m, csr.block_n))
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
-    rc = lib.saf_bsa_bwd(tdo, ctypes.byref(tq), ctypes.byref(tk), tv, to, lse.data_ptr(), lse.stride(1), tdq, tdk,
-                         tdv, csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
-                         csr.block_n, float(sm_scale), ws.data_ptr(), ws.numel(), _stream_ptr(dev))
-    _lib.check("saf_bsa_bwd", rc)
+    tq, tk = _p4(q), _p4(k)
+    ws_bytes = lib.saf_bsa_bwd_workspace_bytes(tq, tk, csr.block_m, csr.block_n)
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
+    rc = lib.saf_bsa_bwd(_p4(dout), tq, tk, _p4(v), _p4(out), lse.data_ptr(), lh, _p4(dq), _p4(dk), _p4(dv),
+                         csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
+                         csr.block_n, sm_scale, ws.data_ptr(), ws_bytes, _stream_ptr(dev))
+    if rc:
+        _lib.check("saf_bsa_bwd", rc)
     return dq, dk, dv
 
 
@@ -496,41 +517,44 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: tor
     gradient.  ``k`` may have another head count, or be None.  ``out``: the
     pair of results (q and k themselves to rotate in place).  Returns
     ``(q', k')``, or ``q'`` when ``k`` is None (saf_rope)."""
-    given = (q,) if k is None else (q, k)
-    dev = _require_cuda(*given, cos, sin)
-    if layout not in _ROPE_LAYOUTS:
+    half = _ROPE_LAYOUTS.get(layout)
+    if half is None:
         raise ValueError(f"layout must be one of {sorted(_ROPE_LAYOUTS)}, got {layout!r}")
-    if any(x.dim() != 4 for x in given):
-        raise ValueError("q and k must be [B, H, S, D] tensors")
-    if k is not None and (k.dtype != q.dtype or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
-        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more than heads")
+    dev = _device_of(q, cos, sin) if k is None else _device_of(q, k, cos, sin)
+    if q.dim() != 4:
+        raise ValueError(f"q must be a [B, H, S, D] tensor, got shape {tuple(q.shape)}")
     B, _, S, D = q.shape
+    if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more than heads")
     text_len = int(text_len)
     if not 0 <= text_len <= S:
         raise ValueError(f"text_len {text_len} is outside [0, {S}]")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() not in (2, 3):
+    table = cos.shape
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or table != sin.shape or len(table) not in (2, 3):
         raise ValueError("cos and sin must be float32 tensors of one [tokens, R/2] or [B, tokens, R/2] shape")
-    R = 2 * cos.shape[-1]
-    if cos.shape[-2] != S - text_len or (cos.dim() == 3 and cos.shape[0] != B) or not 0 < R <= D:
-        raise ValueError(f"table {tuple(cos.shape)} does not match {S - text_len} rotated tokens of {D} channels")
-    given = tuple(_rows_last(x, 1) for x in given)
+    R = 2 * table[-1]
+    if table[-2] != S - text_len or (len(table) == 3 and table[0] != B) or not 0 < R <= D:
+        raise ValueError(f"table {tuple(table)} does not match {S - text_len} rotated tokens of {D} channels")
+    q = _rows_last(q, 1)
+    if k is not None:
+        k = _rows_last(k, 1)
     if out is None:
-        outs = tuple(torch.empty_like(x) for x in given)
+        oq, ok = torch.empty_like(q), None if k is None else torch.empty_like(k)
     else:
-        outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
-        if len(outs) != len(given) or any(o.shape != x.shape or o.dtype != x.dtype or o.device != dev
-                                          for o, x in zip(outs, given)):
-            raise ValueError("out must match q (and k) in shape, type and device")
-    if q.numel() and given[-1].numel():
+        oq, ok = (out, None) if isinstance(out, torch.Tensor) else out if len(out) == 2 else (None, None)
+        if oq is None or (ok is None) != (k is None):
+            raise ValueError("out must hold one tensor for q and one for k")
+        for o, x in ((oq, q),) if k is None else ((oq, q), (ok, k)):
+            if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device:
+                raise ValueError("out must match q (and k) in shape, type and device")
+    if q.numel() and (k is None or k.numel()):
         cos, sin = cos.contiguous(), sin.contiguous()
-        ts = [_t4(x) for x in given + outs]
-        refs = [ctypes.byref(t) for t in ts]
-        tq, tk, oq, ok = refs if k is not None else (refs[0], None, refs[1], None)
-        rc = _lib.load().saf_rope(tq, tk, oq, ok, cos.data_ptr(), sin.data_ptr(),
-                                  cos.stride(0) if cos.dim() == 3 else 0, text_len, R, _ROPE_LAYOUTS[layout],
-                                  int(inverse), _stream_ptr(dev))
-        _lib.check("saf_rope", rc)
-    return outs[0] if k is None else outs
+        rc = _lib.load().saf_rope(_p4(q), None if k is None else _p4(k), _p4(oq), None if k is None else _p4(ok),
+                                  cos.data_ptr(), sin.data_ptr(), cos.stride(0) if len(table) == 3 else 0, text_len,
+                                  R, half, inverse, _stream_ptr(dev))
+        if rc:
+            _lib.check("saf_rope", rc)
+    return oq if k is None else (oq, ok)
 
 
 def permute_tokens(x: torch.Tensor, perm: torch.Tensor, heads: Optional[torch.Tensor] = None,
