@@ -18,6 +18,7 @@ int32_t bsa_bwd_sm100(const saf_tensor4* dout, const saf_tensor4* q, const saf_t
 namespace {
 
 constexpr int kT = 64;            // sub-tile edge of the CUDA-core kernel
+constexpr int kSimtThreads = 256;
 constexpr int kGroup = 32;        // mask lines one list block handles
 constexpr int kRowChunk = 128;    // rows one statistics block handles
 constexpr int kMaxBlocks = 16384; // 14-bit block indexes in the lists
@@ -25,6 +26,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // Mask lines that share a tile: 64-token blocks pair up under the 16-bit kernel.
 int merge_of(int32_t dtype, int block) { return dtype != SAF_F32 && block == 64 ? 2 : 1; }
+
+int simt_chunks(int64_t tiles);
 
 BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, uint8_t* base) {
   BwdWorkspace w{};
@@ -54,6 +57,14 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
     w.class_count = reinterpret_cast<int32_t*>(take((kClasses + 1) * 4));
     w.next = w.class_count + kClasses;
     w.amax = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (w.Sp / 128)) * 4));
+  }
+  if (q->dtype == SAF_F32) {
+    const int64_t tk = (k->S + kT - 1) / kT, tq = (q->S + kT - 1) / kT;
+    w.chunks = simt_chunks(BH * (tk + tq));
+    if (w.chunks > 1) {
+      w.part = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (2 * tk + tq)) * w.chunks * kT * q->D * 4));
+      w.part_count = reinterpret_cast<int*>(take(static_cast<size_t>(BH * (tk + tq)) * 4));
+    }
   }
   w.bytes = at;
   return w;
@@ -232,14 +243,22 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
       }
     }
   } else {
-    for (int r = warp; r < kRowChunk; r += 8) {
-      const int row = chunk * kRowChunk + r;
-      float sum = 0.f;
-      if (row < p.Sq)
-        for (int e = lane; e < p.D; e += 32) sum = fmaf(o[row * p.o_ss + e], d[row * p.d_ss + e], sum);
+    // a warp's 16 rows, four at a time in flight
+    for (int r0 = warp; r0 < kRowChunk; r0 += 32) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int e = lane; e < p.D; e += 32)
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      if (lane == 0) store(row, sum);
+        for (int i = 0; i < 4; ++i) {
+          const int row = chunk * kRowChunk + r0 + 8 * i;
+          if (row < p.Sq) sum[i] = fmaf(o[row * p.o_ss + e], d[row * p.d_ss + e], sum[i]);
+        }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], off);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane == 0) store(chunk * kRowChunk + r0 + 8 * i, sum[i]);
     }
   }
 }
@@ -266,15 +285,45 @@ struct SimtBwdParams {
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
   int H, Sq, Sk, bm, bn, tiles_k;
   float scale;
+  bool vec;  // every row of q, k, v, dout starts at a multiple of 16 bytes
+  int chunks, part_tiles;  // CTAs a tile; partial tiles a head (two a key tile, one a query tile)
+  float* part;
+  int* part_count;  // [BH, tiles]
   BwdWorkspace w;
 };
 
-// Rows [r0, r0 + 64) of a [S, D] view into dst [64][D + 4]; zeros past S.
+// Rows [r0, r0 + 64) of two [S, D] views into dst1 and dst2 [64][D + 4], zeros
+// past S; all of a thread's loads of a pass are in flight before its stores.
+// vec: every row starts at a multiple of 16 bytes.
 template <int D>
-__device__ __forceinline__ void load_tile(float* dst, const float* src, int64_t ss, int r0, int S) {
-  for (int i = threadIdx.x; i < kT * D; i += 256) {
-    const int r = i / D, d = i % D;
-    dst[r * (D + 4) + d] = r0 + r < S ? src[(r0 + r) * ss + d] : 0.f;
+__device__ __forceinline__ void load_tiles(float* dst1, const float* src1, int64_t ss1, float* dst2, const float* src2,
+                                           int64_t ss2, int r0, int S, bool vec) {
+  if (vec) {
+    constexpr int kPass = 4;
+#pragma unroll
+    for (int j0 = 0; j0 < kT * D / 4 / kSimtThreads; j0 += kPass) {
+      float4 x[kPass], y[kPass];
+#pragma unroll
+      for (int j = 0; j < kPass; ++j) {
+        const int i = threadIdx.x + (j0 + j) * kSimtThreads, r = i / (D / 4), d = i % (D / 4) * 4;
+        const bool in = r0 + r < S;
+        x[j] = in ? *reinterpret_cast<const float4*>(src1 + (r0 + r) * ss1 + d) : float4{0.f, 0.f, 0.f, 0.f};
+        y[j] = in ? *reinterpret_cast<const float4*>(src2 + (r0 + r) * ss2 + d) : float4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int j = 0; j < kPass; ++j) {
+        const int i = threadIdx.x + (j0 + j) * kSimtThreads, r = i / (D / 4), d = i % (D / 4) * 4;
+        *reinterpret_cast<float4*>(dst1 + r * (D + 4) + d) = x[j];
+        *reinterpret_cast<float4*>(dst2 + r * (D + 4) + d) = y[j];
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < kT * D; i += kSimtThreads) {
+      const int r = i / D, d = i % D;
+      const bool in = r0 + r < S;
+      dst1[r * (D + 4) + d] = in ? src1[(r0 + r) * ss1 + d] : 0.f;
+      dst2[r * (D + 4) + d] = in ? src2[(r0 + r) * ss2 + d] : 0.f;
+    }
   }
 }
 
@@ -282,20 +331,35 @@ __device__ __forceinline__ float dot4(float4 a, float4 b, float c) {
   return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, c))));
 }
 
-// One CTA per 64 output rows: key rows (dk and dv) for blockIdx.x < tiles_k,
+template <int D>
+constexpr int kSimtSmem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
+
+// CTAs that share a tile's walk, sub-tile by sub-tile in turn: with few tiles
+// one CTA a tile leaves the GPU idle behind the longest list.  Enough for four
+// CTAs an SM, at most 8; from 592 tiles on there is no split.  (Two heads of
+// 32 tiles each way at 2048 tokens: 200 us unsplit.)
+int simt_chunks(int64_t tiles) {
+  const int64_t want = (4 * 148 + tiles - 1) / tiles;
+  return static_cast<int>(want < 1 ? 1 : want > 8 ? 8 : want);
+}
+
+// p.chunks CTAs per 64 output rows: key rows (dk and dv) for tile < tiles_k,
 // query rows (dq) after them.  The tile's own two operands (k, v or q, do)
 // stay in shared memory; the walk brings the other two.  Thread (ty, tx) of a
 // 16 x 16 grid forms the scores of walked rows ty + 16a against own rows
-// tx + 16c, then owns output rows ty*4..+3, channels tx*4..+3 (twice at D = 128).
+// tx + 16c, then owns output rows ty*4..+3, channels tx*4..+3 (twice at
+// D = 128).  The partial sums of a split tile go to the workspace; the CTA
+// that finishes last adds them in the order of the chunks.  Bound by
+// shared-memory reads and the FMA pipe.
 template <int D, bool kKeys>
-__device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
+__device__ void simt_tile(const SimtBwdParams& p, int g, int tile, int chunk) {
   constexpr int LD = D + 4, DC = D / 64;
   extern __shared__ float smf[];
-  float* a1 = smf;               // own k or q
-  float* a2 = a1 + kT * LD;      // own v or do
-  float* b1 = a2 + kT * LD;      // walked q or k
-  float* b2 = b1 + kT * LD;      // walked do or v
-  float* ps = b2 + kT * LD;      // [walked row][own row] p
+  float* a1 = smf;                                // own k or q
+  float* a2 = a1 + kT * LD;                       // own v or do
+  float* b1 = a2 + kT * LD;                       // walked q or k
+  float* b2 = b1 + kT * LD;                       // walked do or v
+  float* ps = b2 + kT * LD;                       // [walked row][own row] p
   float* ds = ps + kT * (kT + 4);
   float* sl = ds + kT * (kT + 4);  // [64] -lse of the tile's or the walked query rows
   float* sd = sl + kT;             // [64] -delta
@@ -308,8 +372,8 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
   const int own0 = tile * kT;
   const float* lse_g = p.w.stat_lse + static_cast<int64_t>(g) * p.w.Sp;
   const float* delta_g = p.w.stat_delta + static_cast<int64_t>(g) * p.w.Sp;
-  load_tile<D>(a1, kKeys ? kg : qg, kKeys ? p.k_ss : p.q_ss, own0, kKeys ? p.Sk : p.Sq);
-  load_tile<D>(a2, kKeys ? vg : dg, kKeys ? p.v_ss : p.do_ss, own0, kKeys ? p.Sk : p.Sq);
+  load_tiles<D>(a1, kKeys ? kg : qg, kKeys ? p.k_ss : p.q_ss, a2, kKeys ? vg : dg, kKeys ? p.v_ss : p.do_ss, own0,
+                kKeys ? p.Sk : p.Sq, p.vec);
   if (!kKeys && tid < kT) {
     sl[tid] = lse_g[own0 + tid];
     sd[tid] = delta_g[own0 + tid];
@@ -327,82 +391,133 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
   const int lines = kKeys ? p.w.lines_k : p.w.lines_q, cap = kKeys ? p.w.cap_k : p.w.cap_q;
   const int64_t at = static_cast<int64_t>(g) * lines + line;
   const uint16_t* list = (kKeys ? p.w.list_k : p.w.list_q) + at * cap;
-  const int n = (kKeys ? p.w.count_k : p.w.count_q)[at];
-  const int walk_len = kKeys ? p.Sq : p.Sk;
-  for (int e = 0; e < n; ++e) {
-    for (int w0 = (list[e] & 0x3fff) * walk_block, w1 = w0 + walk_block; w0 < w1 && w0 < walk_len; w0 += kT) {
-      __syncthreads();  // the previous step is consumed
-      load_tile<D>(b1, kKeys ? qg : kg, kKeys ? p.q_ss : p.k_ss, w0, walk_len);
-      load_tile<D>(b2, kKeys ? dg : vg, kKeys ? p.do_ss : p.v_ss, w0, walk_len);
-      if (kKeys && tid < kT) {
-        sl[tid] = lse_g[w0 + tid];
-        sd[tid] = delta_g[w0 + tid];
-      }
-      __syncthreads();
-      float s[4][4], dp[4][4];
+  const int walk_len = kKeys ? p.Sq : p.Sk, subs = walk_block / kT;
+  const int steps = (kKeys ? p.w.count_k : p.w.count_q)[at] * subs;  // sub-tiles of 64 walked rows
+  for (int st = chunk; st < steps; st += p.chunks) {
+    const int w0 = (list[st / subs] & 0x3fff) * walk_block + st % subs * kT;
+    if (w0 >= walk_len) continue;  // past the end of the last block
+    __syncthreads();  // the previous step is consumed
+    load_tiles<D>(b1, kKeys ? qg : kg, kKeys ? p.q_ss : p.k_ss, b2, kKeys ? dg : vg, kKeys ? p.do_ss : p.v_ss, w0,
+                  walk_len, p.vec);
+    if (kKeys && tid < kT) {
+      sl[tid] = lse_g[w0 + tid];
+      sd[tid] = delta_g[w0 + tid];
+    }
+    __syncthreads();
+    float s[4][4], dp[4][4];
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+    for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[a][c] = dp[a][c] = 0.f;
-      for (int d = 0; d < D; d += 4) {
-        float4 x[4], y[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          x[c] = *reinterpret_cast<const float4*>(&b1[(ty + 16 * c) * LD + d]);
-          y[c] = *reinterpret_cast<const float4*>(&a1[(tx + 16 * c) * LD + d]);
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[a][c] = dot4(x[a], y[c], s[a][c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          x[c] = *reinterpret_cast<const float4*>(&b2[(ty + 16 * c) * LD + d]);
-          y[c] = *reinterpret_cast<const float4*>(&a2[(tx + 16 * c) * LD + d]);
-        }
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) dp[a][c] = dot4(x[a], y[c], dp[a][c]);
-      }
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int wr = ty + 16 * a, orow = tx + 16 * c;
-          const int qi = kKeys ? wr : orow, key = kKeys ? own0 + orow : w0 + wr;
-          // keys past the end (zeros in shared memory) give nothing
-          const bool in = key < p.Sk && sl[qi] != -INFINITY;
-          const float pr = in ? expf(fmaf(s[a][c], p.scale, sl[qi])) : 0.f;
-          if (kKeys) ps[wr * (kT + 4) + orow] = pr;
-          ds[wr * (kT + 4) + orow] = in ? pr * (dp[a][c] + sd[qi]) : 0.f;
-        }
-      __syncthreads();
+      for (int c = 0; c < 4; ++c) s[a][c] = dp[a][c] = 0.f;
 #pragma unroll 4
-      for (int w = 0; w < kT; ++w) {
-        const float4 m = *reinterpret_cast<const float4*>(&ds[w * (kT + 4) + ty * 4]);
-        const float mv[4] = {m.x, m.y, m.z, m.w};
-        float pv[4];
-        if (kKeys) {
-          const float4 pm = *reinterpret_cast<const float4*>(&ps[w * (kT + 4) + ty * 4]);
-          pv[0] = pm.x, pv[1] = pm.y, pv[2] = pm.z, pv[3] = pm.w;
-        }
+    for (int d = 0; d < D; d += 4) {
+      float4 x[4], y[4];
 #pragma unroll
-        for (int dc = 0; dc < DC; ++dc) {
-          const float4 x = *reinterpret_cast<const float4*>(&b1[w * LD + dc * 64 + tx * 4]);
-          const float xv[4] = {x.x, x.y, x.z, x.w};
+      for (int c = 0; c < 4; ++c) {
+        x[c] = *reinterpret_cast<const float4*>(&b1[(ty + 16 * c) * LD + d]);
+        y[c] = *reinterpret_cast<const float4*>(&a1[(tx + 16 * c) * LD + d]);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[a][c] = dot4(x[a], y[c], s[a][c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[c] = *reinterpret_cast<const float4*>(&b2[(ty + 16 * c) * LD + d]);
+        y[c] = *reinterpret_cast<const float4*>(&a2[(tx + 16 * c) * LD + d]);
+      }
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) dp[a][c] = dot4(x[a], y[c], dp[a][c]);
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int wr = ty + 16 * a, orow = tx + 16 * c;
+        const int qi = kKeys ? wr : orow, key = kKeys ? own0 + orow : w0 + wr;
+        // keys past the end (zeros in shared memory) give nothing
+        const bool in = key < p.Sk && sl[qi] != -INFINITY;
+        const float pr = in ? expf(fmaf(s[a][c], p.scale, sl[qi])) : 0.f;
+        if (kKeys) ps[wr * (kT + 4) + orow] = pr;
+        ds[wr * (kT + 4) + orow] = in ? pr * (dp[a][c] + sd[qi]) : 0.f;
+      }
+    __syncthreads();
+#pragma unroll 4
+    for (int w = 0; w < kT; ++w) {
+      const float4 m = *reinterpret_cast<const float4*>(&ds[w * (kT + 4) + ty * 4]);
+      const float mv[4] = {m.x, m.y, m.z, m.w};
+      float pv[4];
+      if (kKeys) {
+        const float4 pm = *reinterpret_cast<const float4*>(&ps[w * (kT + 4) + ty * 4]);
+        pv[0] = pm.x, pv[1] = pm.y, pv[2] = pm.z, pv[3] = pm.w;
+      }
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc) {
+        const float4 x = *reinterpret_cast<const float4*>(&b1[w * LD + dc * 64 + tx * 4]);
+        const float xv[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc1[i][dc * 4 + c] = fmaf(mv[i], xv[c], acc1[i][dc * 4 + c]);
+        if (kKeys) {
+          const float4 y = *reinterpret_cast<const float4*>(&b2[w * LD + dc * 64 + tx * 4]);
+          const float yv[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc1[i][dc * 4 + c] = fmaf(mv[i], xv[c], acc1[i][dc * 4 + c]);
-          if (kKeys) {
-            const float4 y = *reinterpret_cast<const float4*>(&b2[w * LD + dc * 64 + tx * 4]);
-            const float yv[4] = {y.x, y.y, y.z, y.w};
+            for (int c = 0; c < 4; ++c) acc2[i][dc * 4 + c] = fmaf(pv[i], yv[c], acc2[i][dc * 4 + c]);
+        }
+      }
+    }
+  }
+  if (p.chunks > 1) {
+    constexpr int kPart = kT * D;
+    float* part = p.part + ((static_cast<int64_t>(g) * p.part_tiles + (kKeys ? 2 * tile : 2 * p.tiles_k + tile)) * p.chunks) *
+                               kPart;
+    // [chunk][dk or dq], then for keys [chunk][dv]; each thread's values side by side
+    float4* mine1 = reinterpret_cast<float4*>(part + chunk * kPart) + tid * (4 * DC);
+    float4* mine2 = mine1 + static_cast<int64_t>(p.chunks) * kPart / 4;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) acc2[i][dc * 4 + c] = fmaf(pv[i], yv[c], acc2[i][dc * 4 + c]);
-          }
+      for (int c = 0; c < DC; ++c) {
+        mine1[i * DC + c] = make_float4(acc1[i][4 * c], acc1[i][4 * c + 1], acc1[i][4 * c + 2], acc1[i][4 * c + 3]);
+        if (kKeys)
+          mine2[i * DC + c] = make_float4(acc2[i][4 * c], acc2[i][4 * c + 1], acc2[i][4 * c + 2], acc2[i][4 * c + 3]);
+      }
+    __threadfence();
+    __syncthreads();
+    __shared__ int last;
+    if (tid == 0)
+      last = atomicAdd(p.part_count + static_cast<int64_t>(g) * gridDim.x + blockIdx.x, 1) == p.chunks - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 4 * DC; ++c) {
+        acc1[i][c] = 0.f;
+        if (kKeys) acc2[i][c] = 0.f;
+      }
+    for (int ch = 0; ch < p.chunks; ++ch) {  // a chunk's values are in flight together
+      const float4* at1 = reinterpret_cast<const float4*>(part + ch * kPart) + tid * (4 * DC);
+      const float4* at2 = at1 + static_cast<int64_t>(p.chunks) * kPart / 4;
+      float4 x[4 * DC], y[kKeys ? 4 * DC : 1];
+#pragma unroll
+      for (int j = 0; j < 4 * DC; ++j) {
+        x[j] = __ldcg(at1 + j);
+        if (kKeys) y[j] = __ldcg(at2 + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 4 * DC; ++j) {
+        float* a = &acc1[j / DC][j % DC * 4];
+        a[0] += x[j].x, a[1] += x[j].y, a[2] += x[j].z, a[3] += x[j].w;
+        if (kKeys) {
+          float* v = &acc2[j / DC][j % DC * 4];
+          v[0] += y[j].x, v[1] += y[j].y, v[2] += y[j].z, v[3] += y[j].w;
         }
       }
     }
@@ -424,19 +539,19 @@ __device__ void simt_tile(const SimtBwdParams& p, int g, int tile) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(256) bsa_bwd_simt_kernel(const SimtBwdParams p) {
+__global__ void __launch_bounds__(kSimtThreads, D == 64 ? 2 : 1) bsa_bwd_simt_kernel(const SimtBwdParams p) {
   if (static_cast<int>(blockIdx.x) < p.tiles_k)
-    simt_tile<D, true>(p, blockIdx.y, blockIdx.x);
+    simt_tile<D, true>(p, blockIdx.y, blockIdx.x, blockIdx.z);
   else
-    simt_tile<D, false>(p, blockIdx.y, blockIdx.x - p.tiles_k);
+    simt_tile<D, false>(p, blockIdx.y, blockIdx.x - p.tiles_k, blockIdx.z);
 }
 
 template <int D>
 int32_t launch_simt(const SimtBwdParams& p, int tiles_q, int BH, cudaStream_t st) {
-  const int smem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
-  if (const int32_t rc = allow_smem<bsa_bwd_simt_kernel<D>>(smem); rc != SAF_OK) return rc;
-  const dim3 grid(static_cast<unsigned>(p.tiles_k + tiles_q), static_cast<unsigned>(BH));
-  bsa_bwd_simt_kernel<D><<<grid, 256, smem, st>>>(p);
+  if (const int32_t rc = allow_smem<bsa_bwd_simt_kernel<D>>(kSimtSmem<D>); rc != SAF_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(p.tiles_k + tiles_q), static_cast<unsigned>(BH),
+                  static_cast<unsigned>(p.chunks));
+  bsa_bwd_simt_kernel<D><<<grid, kSimtThreads, kSimtSmem<D>, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
 }
@@ -553,6 +668,14 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
   sp.tiles_k = static_cast<int>((k->S + kT - 1) / kT);
   const int tiles_q = static_cast<int>((q->S + kT - 1) / kT);
   sp.scale = sm_scale;
+  sp.vec = true;
+  for (const saf_tensor4* t : {q, k, v, dout})
+    sp.vec = sp.vec && (reinterpret_cast<uintptr_t>(t->data) & 15) == 0 && t->stride_s % 4 == 0 &&
+             (t->H == 1 || t->stride_h % 4 == 0) && (t->B == 1 || t->stride_b % 4 == 0);
   sp.w = pp.w;
+  sp.chunks = pp.w.chunks, sp.part = pp.w.part, sp.part_count = pp.w.part_count;
+  sp.part_tiles = 2 * sp.tiles_k + tiles_q;
+  if (sp.chunks > 1)
+    SAF_CUDA_TRY(cudaMemsetAsync(sp.part_count, 0, static_cast<size_t>(BH) * (sp.tiles_k + tiles_q) * sizeof(int), st));
   return q->D == 64 ? launch_simt<64>(sp, tiles_q, BH, st) : launch_simt<128>(sp, tiles_q, BH, st);
 }

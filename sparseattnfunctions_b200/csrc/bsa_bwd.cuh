@@ -34,6 +34,11 @@ struct BwdWorkspace {
   int32_t* class_count;  // [kClasses]
   int32_t* next;         // the next item to take
   float* amax;           // [BH, Sp / 128]
+  // fp32 kernel only, when several CTAs share a tile: their partial sums and
+  // the tiles' counts of finished CTAs
+  int chunks;
+  float* part;
+  int* part_count;
   int lines_q, lines_k, cap_q, cap_k;
   int64_t Sp;  // Sq rounded up to 128
   size_t bytes;

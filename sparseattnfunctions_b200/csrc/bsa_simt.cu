@@ -26,6 +26,7 @@ int32_t bsa_fwd_sm100_keys(const saf_tensor4* q, const saf_tensor4* k, const saf
 namespace {
 
 constexpr int kT = 64;  // sub-tile edge
+constexpr int kMaxChunks = 8;  // CTAs that may share a tile of the training forward
 
 struct SimtParams {
   const float* q;
@@ -44,20 +45,56 @@ struct SimtParams {
   unsigned int* status;
   const int4* row_ranges;  // nullable [Sq]: key intervals [x, y) U [z, w) of each query row
   float* lse;  // nullable [B*H, Sq]: row log-sum-exp; rows without a live key then give zeros
+  // training forward: gridDim.z CTAs share a tile's key sub-tiles, one by one
+  // in turn; partial O, m, l per row [B*H, tiles, chunks, 64, D + 2], and the
+  // tiles' counts of finished CTAs (zero on entry)
+  int chunks;
+  bool vec;  // every row of q, k, v starts at a multiple of 16 bytes
+  float* part;
+  int* part_count;
 };
 
+// Rows [r0, r0 + 64) of a [S, D] view into dst [64][LD], zeros past S; all of a
+// thread's loads are in flight before its first store.  vec: every row starts
+// at a multiple of 16 bytes.
+template <int D, int LD>
+__device__ __forceinline__ void fwd_tile(float* dst, const float* src, int64_t ss, int r0, int S, bool vec) {
+  constexpr int N = kT * D / 4 / 256;
+  if (vec) {
+    float4 x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = threadIdx.x + j * 256, r = i / (D / 4), d = i % (D / 4) * 4;
+      x[j] = r0 + r < S ? *reinterpret_cast<const float4*>(src + (r0 + r) * ss + d) : float4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = threadIdx.x + j * 256, r = i / (D / 4), d = i % (D / 4) * 4;
+      *reinterpret_cast<float4*>(dst + r * LD + d) = x[j];
+    }
+  } else {
+    for (int i = threadIdx.x; i < kT * D; i += 256) {
+      const int r = i / D, d = i % D;
+      dst[r * LD + d] = r0 + r < S ? src[(r0 + r) * ss + d] : 0.f;
+    }
+  }
+}
+
 // grid (ceil(Sq/64), B*H), 256 threads.  Thread (ty, tx) in a 16 x 16 grid
-// owns S rows ty*4..+3, columns tx*4..+3, and O rows ty*4..+3,
-// columns tx*(D/16)..+D/16.
+// owns S rows ty*4..+3, columns tx + 16c, and O rows ty*4..+3, columns
+// tx*(D/16)..+D/16.  Tiles lie row by row with padded rows, so that they are
+// written and read 16 bytes a thread without bank conflicts (a transposed
+// tile's stores ran 32 to a bank: 8 key blocks at 2048 tokens took 90 us).
 template <int D>
 __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
   constexpr int DC = D / 16;  // O columns per thread
   extern __shared__ float sm[];
-  float* qt = sm;                // [D][64]  (q transposed)
-  float* kt = qt + D * kT;       // [D][64]  (k transposed)
-  float* vs = kt + D * kT;       // [64][D]
-  float* ss = vs + kT * D;       // [64][65] scores / probabilities
-  float* alpha_s = ss + kT * (kT + 1);  // [64]
+  constexpr int LD = D + 4, LS = kT + 4;
+  float* qs = sm;                // [64][D + 4]
+  float* ks = qs + kT * LD;      // [64][D + 4]
+  float* vs = ks + kT * LD;      // [64][D]
+  float* ss = vs + kT * D;       // [64][68] scores / probabilities
+  float* alpha_s = ss + kT * LS;        // [64]
   float* bias_s = alpha_s + kT;         // [64]
 
   const int tile = blockIdx.x, g = blockIdx.y;
@@ -68,11 +105,7 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
   const float* kg = p.k + b * p.k_sb + h * p.k_sh;
   const float* vg = p.v + b * p.v_sb + h * p.v_sh;
 
-  for (int idx = tid; idx < kT * D; idx += 256) {
-    const int r = idx / D, d = idx % D;
-    const int row = q0 + r;
-    qt[d * kT + r] = row < p.Sq ? qg[static_cast<int64_t>(row) * p.q_ss + d] : 0.f;
-  }
+  fwd_tile<D, LD>(qs, qg, p.q_ss, q0, p.Sq, p.vec);
 
   float acc[4][DC];
 #pragma unroll
@@ -95,22 +128,19 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
   };
   const int64_t e_beg = clampi(rp[mrow]), e_end = clampi(rp[mrow + 1]);
   const int subs = p.bn / kT;
-  for (int64_t e = e_beg; e < e_end; ++e) {
-    const int col = p.col_idx[e];
+  const int64_t steps = (e_end - e_beg) * subs;  // 64-key sub-tiles
+  for (int64_t st = blockIdx.z; st < steps; st += p.chunks) {
+    const int col = p.col_idx[e_beg + st / subs];
     if (col < 0 || col >= p.nbk) {
       if (tid == 0) atomicOr(p.status, SAF_DEV_BADINDEX);
       continue;
     }
-    for (int u = 0; u < subs; ++u) {
-      const int k0 = col * p.bn + u * kT;
-      if (k0 >= p.Sk) break;
+    {
+      const int k0 = col * p.bn + static_cast<int>(st % subs) * kT;
+      if (k0 >= p.Sk) continue;
       __syncthreads();  // previous tile fully consumed
-      for (int idx = tid; idx < kT * D; idx += 256) {
-        const int r = idx / D, d = idx % D;
-        const int row = k0 + r;
-        kt[d * kT + r] = row < p.Sk ? kg[static_cast<int64_t>(row) * p.k_ss + d] : 0.f;
-        vs[r * D + d] = row < p.Sk ? vg[static_cast<int64_t>(row) * p.v_ss + d] : 0.f;
-      }
+      fwd_tile<D, LD>(ks, kg, p.k_ss, k0, p.Sk, p.vec);
+      fwd_tile<D, D>(vs, vg, p.v_ss, k0, p.Sk, p.vec);
       if (tid < kT) {
         const int row = k0 + tid;
         bias_s[tid] = (p.kv_bias != nullptr && row < p.Sk)
@@ -124,20 +154,29 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[i][c] = 0.f;
-      for (int d = 0; d < D; ++d) {
-        const float4 a = *reinterpret_cast<const float4*>(&qt[d * kT + ty * 4]);
-        const float4 bb = *reinterpret_cast<const float4*>(&kt[d * kT + tx * 4]);
-        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {bb.x, bb.y, bb.z, bb.w};
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 a[4], bb[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          a[c] = *reinterpret_cast<const float4*>(&qs[(ty * 4 + c) * LD + d]);
+          bb[c] = *reinterpret_cast<const float4*>(&ks[(tx + 16 * c) * LD + d]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[i][c] = fmaf(av[i], bv[c], s[i][c]);
+          for (int c = 0; c < 4; ++c) {  // ascending d
+            s[i][c] = fmaf(a[i].x, bb[c].x, s[i][c]);
+            s[i][c] = fmaf(a[i].y, bb[c].y, s[i][c]);
+            s[i][c] = fmaf(a[i].z, bb[c].z, s[i][c]);
+            s[i][c] = fmaf(a[i].w, bb[c].w, s[i][c]);
+          }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int kc = tx * 4 + c;
+          const int kc = tx + 16 * c;
           bool keep = k0 + kc < p.Sk;
           if (p.row_ranges != nullptr) {
             const int qr = q0 + ty * 4 + i, kk = k0 + kc;
@@ -146,7 +185,7 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
               keep = keep && ((kk >= rr.x && kk < rr.y) || (kk >= rr.z && kk < rr.w));
             }
           }
-          ss[(ty * 4 + i) * (kT + 1) + kc] = keep ? s[i][c] * p.scale + bias_s[kc] : -INFINITY;
+          ss[(ty * 4 + i) * LS + kc] = keep ? s[i][c] * p.scale + bias_s[kc] : -INFINITY;
         }
       __syncthreads();
       // Row softmax update: the 16 threads of row group ty split the columns.
@@ -154,7 +193,7 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
       for (int i = 0; i < 4; ++i) {
         const int r = ty * 4 + i;
         float mx = -INFINITY;
-        for (int c = tx; c < kT; c += 16) mx = fmaxf(mx, ss[r * (kT + 1) + c]);
+        for (int c = tx; c < kT; c += 16) mx = fmaxf(mx, ss[r * LS + c]);
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         const float m_new = fmaxf(m_run[i], mx);
@@ -162,8 +201,8 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
         const float alpha = expf(m_run[i] - m_safe);
         float sum = 0.f;
         for (int c = tx; c < kT; c += 16) {
-          const float pv = expf(ss[r * (kT + 1) + c] - m_safe);
-          ss[r * (kT + 1) + c] = pv;
+          const float pv = expf(ss[r * LS + c] - m_safe);
+          ss[r * LS + c] = pv;
           sum += pv;
         }
 #pragma unroll
@@ -180,17 +219,82 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
 #pragma unroll
         for (int c = 0; c < DC; ++c) acc[i][c] *= al;
       }
-      for (int kk = 0; kk < kT; ++kk) {
-        float pv[4];
+#pragma unroll 2
+      for (int k4 = 0; k4 < kT; k4 += 4) {
+        float pv[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pv[i] = ss[(ty * 4 + i) * (kT + 1) + kk];
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          const float vv = vs[kk * D + tx * DC + c];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i][c] = fmaf(pv[i], vv, acc[i][c]);
+        for (int i = 0; i < 4; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(&ss[(ty * 4 + i) * LS + k4]);
+          pv[i][0] = x.x, pv[i][1] = x.y, pv[i][2] = x.z, pv[i][3] = x.w;
         }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int c = 0; c < DC; ++c) {
+            const float vv = vs[(k4 + kk) * D + tx * DC + c];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i][c] = fmaf(pv[i][kk], vv, acc[i][c]);
+          }
       }
+    }
+  }
+  if (p.chunks > 1) {  // the CTA that finishes last merges the tile's partial rows, in the chunks' order
+    constexpr int kRow = D + 2;
+    const int64_t at = static_cast<int64_t>(g) * gridDim.x + tile;
+    float* part = p.part + at * p.chunks * (kT * kRow);
+    float* mine = part + blockIdx.z * (kT * kRow);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float* r = mine + (ty * 4 + i) * kRow;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) r[tx * DC + c] = acc[i][c];
+      if (tx == 0) r[D] = m_run[i], r[D + 1] = l_run[i];
+    }
+    __threadfence();
+    __syncthreads();
+    __shared__ int last;
+    if (tid == 0) last = atomicAdd(p.part_count + at, 1) == p.chunks - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    // every chunk's maxima and sums first, then its rows, each set of loads in flight together
+    float mc[4][kMaxChunks], lc[4][kMaxChunks];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int ch = 0; ch < kMaxChunks; ++ch) {
+        const float* r = part + (ch * kT + ty * 4 + i) * kRow + D;
+        mc[i][ch] = ch < p.chunks ? __ldcg(r) : -INFINITY;
+        lc[i][ch] = ch < p.chunks ? __ldcg(r + 1) : 0.f;
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int ch = 0; ch < kMaxChunks; ++ch) m = fmaxf(m, mc[i][ch]);
+#pragma unroll
+      for (int ch = 0; ch < kMaxChunks; ++ch) {
+        mc[i][ch] = mc[i][ch] == -INFINITY ? 0.f : expf(mc[i][ch] - m);  // the chunk's weight; -inf: no key seen
+        l += lc[i][ch] * mc[i][ch];
+      }
+      m_run[i] = m;
+      l_run[i] = l;
+#pragma unroll
+      for (int c = 0; c < DC; ++c) acc[i][c] = 0.f;
+    }
+#pragma unroll
+    for (int ch = 0; ch < kMaxChunks; ++ch) {
+      if (ch >= p.chunks) break;
+      float x[4][DC];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < DC; ++c) x[i][c] = __ldcg(part + (ch * kT + ty * 4 + i) * kRow + tx * DC + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          if (mc[i][ch] != 0.f) acc[i][c] += x[i][c] * mc[i][ch];
     }
   }
 #pragma unroll
@@ -207,10 +311,17 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
   }
 }
 
+// CTAs a 64-row tile of the training forward: four tiles' worth of CTAs an SM,
+// at most 8 a tile (64 tiles of 8 key blocks at 2048 tokens: 90 us unsplit).
+int simt_chunks(int64_t tiles) {
+  const int64_t want = (4 * 148 + tiles - 1) / tiles;
+  return static_cast<int>(want < 1 ? 1 : want > kMaxChunks ? kMaxChunks : want);
+}
+
 int32_t bsa_fwd_simt(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                      const saf_tensor4* o, const int32_t* row_ptr, const int32_t* col_idx,
                      int64_t col_capacity, int bm, int bn, const float* kv_bias,
-                     int64_t bias_stride, float sm_scale, const int32_t* row_ranges, float* lse,
+                     int64_t bias_stride, float sm_scale, const int32_t* row_ranges, const TrainArgs* train,
                      cudaStream_t stream) {
   if (bm % kT != 0 || bn % kT != 0) return SAF_ERR_UNSUPPORTED;
   if (q->D != 64 && q->D != 128) return SAF_ERR_UNSUPPORTED;
@@ -237,16 +348,29 @@ int32_t bsa_fwd_simt(const saf_tensor4* q, const saf_tensor4* k, const saf_tenso
   p.bias_stride = bias_stride;
   p.scale = sm_scale;
   p.row_ranges = reinterpret_cast<const int4*>(row_ranges);
-  p.lse = lse;
+  p.lse = train != nullptr ? train->lse : nullptr;
+  p.chunks = 1;
+  p.vec = true;
+  for (const saf_tensor4* t : {q, k, v})
+    p.vec = p.vec && (reinterpret_cast<uintptr_t>(t->data) & 15) == 0 && t->stride_s % 4 == 0 &&
+            (t->H == 1 || t->stride_h % 4 == 0) && (t->B == 1 || t->stride_b % 4 == 0);
+  if (train != nullptr && train->split_part != nullptr) {
+    const int64_t tiles = q->B * q->H * ((q->S + kT - 1) / kT);
+    p.chunks = simt_chunks(tiles);
+    p.part = train->split_part;
+    p.part_count = train->split_cnt;
+    SAF_CUDA_TRY(cudaMemsetAsync(p.part_count, 0, static_cast<size_t>(tiles) * sizeof(int), stream));
+  }
   p.status = device_status_ptr();
   if (p.status == nullptr) return SAF_ERR_CUDA;
-  dim3 grid(static_cast<unsigned>((q->S + kT - 1) / kT), static_cast<unsigned>(q->B * q->H));
+  dim3 grid(static_cast<unsigned>((q->S + kT - 1) / kT), static_cast<unsigned>(q->B * q->H),
+            static_cast<unsigned>(p.chunks));
   if (q->D == 64) {
-    const int smem = (3 * 64 * kT + kT * (kT + 1) + 2 * kT) * 4;
+    const int smem = (2 * kT * (64 + 4) + 64 * kT + kT * (kT + 4) + 2 * kT) * 4;
     if (const int32_t rc = allow_smem<bsa_fwd_simt_kernel<64>>(smem); rc != SAF_OK) return rc;
     bsa_fwd_simt_kernel<64><<<grid, 256, smem, stream>>>(p);
   } else {
-    const int smem = (3 * 128 * kT + kT * (kT + 1) + 2 * kT) * 4;
+    const int smem = (2 * kT * (128 + 4) + 128 * kT + kT * (kT + 4) + 2 * kT) * 4;
     if (const int32_t rc = allow_smem<bsa_fwd_simt_kernel<128>>(smem); rc != SAF_OK) return rc;
     bsa_fwd_simt_kernel<128><<<grid, 256, smem, stream>>>(p);
   }
@@ -304,7 +428,7 @@ int32_t bsa_fwd_entry(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
     DeviceScope dev_scope;
     if ((rc = dev_scope.bind(q->data)) != SAF_OK) return rc;
     return bsa_fwd_simt(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, kv_bias,
-                        kv_bias_stride_bh, sm_scale, row_ranges, train != nullptr ? train->lse : nullptr, st);
+                        kv_bias_stride_bh, sm_scale, row_ranges, train, st);
   }
   // 16-bit path: tcgen05 kernel; tiles of 64 or 128, 16-byte aligned rows.
   if ((block_m != 64 && block_m != 128) || (block_n != 64 && block_n != 128))
@@ -358,15 +482,29 @@ extern "C" int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const
                             kv_bias_stride_bh, sm_scale, lead_rows, nullptr, stream);
 }
 
+// Bytes of a training forward's split buffers (0: every tile runs unsplit).
+static int64_t train_ws_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m, int32_t lead_rows,
+                              int64_t* part_bytes);
+
 static int64_t lead_tiles_of(int32_t lead_rows, int32_t block_m) {
   return (static_cast<int64_t>(lead_rows) * block_m + 127) / 128;
 }
 
 extern "C" size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
                                                  int32_t lead_rows) {
-  if (check_tensor4(q) != SAF_OK || check_tensor4(k) != SAF_OK || block_m <= 0 || lead_rows < 0 || q->dtype == SAF_F32) return 0;
+  if (check_tensor4(q) != SAF_OK || check_tensor4(k) != SAF_OK || block_m <= 0 || lead_rows < 0) return 0;
   int64_t part;
-  return static_cast<size_t>(bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), &part));
+  return static_cast<size_t>(train_ws_bytes(q, k, block_m, lead_rows, &part));
+}
+
+static int64_t train_ws_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m, int32_t lead_rows,
+                              int64_t* part_bytes) {
+  if (q->dtype != SAF_F32)
+    return bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), part_bytes);
+  const int64_t tiles = q->B * q->H * ((q->S + kT - 1) / kT);
+  const int chunks = simt_chunks(tiles);
+  *part_bytes = chunks > 1 ? tiles * chunks * kT * (q->D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
+  return chunks > 1 ? *part_bytes + tiles * static_cast<int64_t>(sizeof(int)) : 0;
 }
 
 extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
@@ -381,15 +519,13 @@ extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, c
   for (const saf_tensor4* t : {k, v, o})
     if ((rc = check_operand(t, q)) != SAF_OK) return rc;
   TrainArgs train{lse, nullptr, nullptr};
-  if (q->dtype != SAF_F32) {
-    int64_t part = 0;
-    const int64_t need = bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), &part);
-    if (need > 0) {
-      if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) return SAF_ERR_WORKSPACE;
-      if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;
-      train.split_part = static_cast<float*>(workspace);
-      train.split_cnt = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + part);
-    }
+  int64_t part = 0;
+  const int64_t need = train_ws_bytes(q, k, block_m, lead_rows, &part);
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) return SAF_ERR_WORKSPACE;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;
+    train.split_part = static_cast<float*>(workspace);
+    train.split_cnt = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + part);
   }
   return bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, nullptr, 0,
                        sm_scale, lead_rows, nullptr, nullptr, nullptr, &train, stream);

@@ -93,8 +93,8 @@ struct PoolArgs {
 };
 
 // Training forward of the attention kernels: the row log-sum-exp output
-// [B*H, Sq] and, for the 16-bit kernel, the caller's buffers for split lead
-// tiles (partial rows and row counters; null when its tiles run unsplit).
+// [B*H, Sq] and the caller's buffers for split tiles: partial rows and counters
+// (null when every tile runs unsplit).
 struct TrainArgs {
   float* lse;
   float* split_part;

@@ -454,7 +454,7 @@ def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR
     lib = _lib.load()
     tq, tk, tv, to = _p4(q), _p4(k), _p4(v), _p4(out)
     lead, ws_bytes, ws_ptr = int(csr.dense_rows), 0, None
-    if lead > 0:
+    if lead > 0 or q.dtype == torch.float32:
         ws_bytes = lib.saf_bsa_fwd_lse_workspace_bytes(tq, tk, csr.block_m, lead)
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)

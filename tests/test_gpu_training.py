@@ -391,10 +391,11 @@ def test_processor_trains(cuda_device, dtype, layout):
     _check_grad((dq, dk, dv), w.cpu(), q.cpu(), k.cpu(), x[2].detach().cpu(), plain.cpu(), lse.cpu(), live, 0.125)
     dq, dk = kernels.rope(dq, dk, table.cos, table.sin, text_len=70, layout=layout, inverse=True)
     assert torch.equal(x[0].grad, dq) and torch.equal(x[1].grad, dk) and torch.equal(x[2].grad, dv)
-    with torch.no_grad():
-        assert torch.equal(attn(*x), out)
+    with torch.no_grad():  # the inference kernel; it may split dense text rows where the training forward does not
+        infer = attn(*x)
+    _check_fwd(infer, lse, q.cpu(), k.cpu(), x[2].detach().cpu(), live, 0.125)
     here = torch.empty_like(out)
-    assert attn(*x, out=here) is here and torch.equal(here, out)
+    assert attn(*x, out=here) is here and torch.equal(here, infer)
 
 
 def test_autograd_of_sums(cuda_device):
