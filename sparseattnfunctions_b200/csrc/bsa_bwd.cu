@@ -23,6 +23,13 @@ constexpr int kGroup = 32;        // mask lines one list block handles
 constexpr int kRowChunk = 128;    // rows one statistics block handles
 constexpr int kMaxBlocks = 16384; // 14-bit block indexes in the lists
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kCounters = kClasses + 3;  // class counts, next item, parts, cut lines
+// A line is cut when it holds more than 1.5 times kMinPart tiles of 128 x 128,
+// and than 1.5 times an SM's share of the work (estimated from its own head's
+// listed blocks); a part holds about that many.  Parts number at most 1.67
+// times the tiles over the share, times up to 4 where 64-token blocks fill
+// tiles sparsely: under kPartCap.
+constexpr int kMinPart = 12, kPartCap = 1024, kMaxParts = 32;
 
 // Mask lines that share a tile: 64-token blocks pair up under the 16-bit kernel.
 int merge_of(int32_t dtype, int block) { return dtype != SAF_F32 && block == 64 ? 2 : 1; }
@@ -52,10 +59,21 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
   w.count_q = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_q) * 4));
   w.count_k = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_k) * 4));
   if (q->dtype != SAF_F32) {
-    const int64_t n = BH * (w.lines_q + w.lines_k);
-    w.items = reinterpret_cast<uint32_t*>(take(static_cast<size_t>(n) * kClasses * 4));
-    w.class_count = reinterpret_cast<int32_t*>(take((kClasses + 1) * 4));
+    // Cutting pays where one list outlasts an SM's share of the whole.  At
+    // 17776 tokens, a tenth of the blocks and dense text, whole and cut lists
+    // take 224 and 98 us at one head, 234 and 137 at two, 235 and 240 at four.
+    const int64_t longest = (q->S > k->S ? q->S : k->S) / 128;
+    w.part_cap = BH <= 3 && 2 * longest > 3 * kMinPart ? kPartCap : 0;
+    w.item_cap = static_cast<int>(BH * (w.lines_q + w.lines_k)) + w.part_cap;
+    w.items = reinterpret_cast<uint2*>(take(static_cast<size_t>(w.item_cap) * kClasses * 8));
+    w.class_count = reinterpret_cast<int32_t*>(take(kCounters * 4));
     w.next = w.class_count + kClasses;
+    w.parts_used = w.next + 1;
+    w.split_count = w.next + 2;
+    if (w.part_cap > 0) {
+      w.part = reinterpret_cast<float*>(take(static_cast<size_t>(w.part_cap) * 2 * 128 * 64 * 4));
+      w.split = reinterpret_cast<uint2*>(take(static_cast<size_t>(w.part_cap / 2) * 8));
+    }
     w.amax = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (w.Sp / 128)) * 4));
   }
   if (q->dtype == SAF_F32) {
@@ -83,7 +101,7 @@ struct PrepParams {
   int64_t lse_stride;  // per head
   float lse_factor, lse_shift;  // stat_lse = lse_shift - lse_factor * lse
   int items;                    // 1: fill the work items
-  int nbq, nbk, merge_q, merge_k;
+  int nbq, nbk, bm, bn, merge_q, merge_k;
   int groups_q, groups_k;
   const int32_t* row_ptr;
   const int32_t* col_idx;
@@ -98,6 +116,7 @@ struct PrepParams {
 __device__ void build_lists(const PrepParams& p, int g, int group, bool columns) {
   extern __shared__ uint32_t sm[];
   __shared__ int cls_n[kClasses], cls_at[kClasses], my_cls[kGroup], my_pos[kGroup];
+  __shared__ uint32_t my_part[kGroup];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int other = columns ? p.nbq : p.nbk, words = (other + 31) >> 5;
   uint32_t* bits = sm;                                       // [32][words]
@@ -166,9 +185,28 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
       const uint32_t id = static_cast<uint32_t>(g * lines + tile);
       count[id] = n;
       if (p.items) {
-        const int cls = kClasses - 1 - (n > 0 ? 31 - __clz(n) : 0);
+        const int other_block = columns ? p.bm : p.bn;
+        const int tiles = other_block == 64 ? (n + 1) / 2 : n;
+        int parts = 1, slot = 0;
+        if (p.w.part_cap > 0) {
+          const int64_t entries = p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1) + p.nbq] -
+                                  p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1)];
+          const int64_t work = 2 * entries * (p.bm * p.bn) / (128 * 128) * gridDim.y;
+          const int64_t share = max(static_cast<int64_t>(kMinPart), (work + 147) / 148);
+          if (2 * static_cast<int64_t>(tiles) > 3 * share) {
+            parts = static_cast<int>(min(static_cast<int64_t>(kMaxParts), (tiles + share - 1) / share));
+            slot = atomicAdd(p.w.parts_used, parts);
+            if (slot + parts > p.w.part_cap) parts = 1, slot = 0;
+          }
+          if (parts > 1)
+            p.w.split[atomicAdd(p.w.split_count, 1)] =
+                make_uint2((columns ? 0x80000000u : 0u) | id, pack_part(slot, 0, parts));
+        }
+        const int len = (tiles + parts - 1) / parts;
+        const int cls = kClasses - 1 - (len > 0 ? 31 - __clz(len) : 0);
         my_cls[t] = cls;
-        my_pos[t] = atomicAdd(&cls_n[cls], 1);
+        my_part[t] = pack_part(slot, 0, parts);
+        my_pos[t] = atomicAdd(&cls_n[cls], parts);
       }
     }
   }
@@ -179,9 +217,11 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
   __syncthreads();
   const int tile = line0 / merge + tid;
   if (tid < kGroup / merge && tile < lines) {
-    const int64_t n_items = static_cast<int64_t>(gridDim.y) * (p.w.lines_q + p.w.lines_k);
-    p.w.items[my_cls[tid] * n_items + cls_at[my_cls[tid]] + my_pos[tid]] =
-        (columns ? 0x80000000u : 0u) | static_cast<uint32_t>(g * lines + tile);
+    uint2* at = p.w.items + static_cast<int64_t>(my_cls[tid]) * p.w.item_cap + cls_at[my_cls[tid]] + my_pos[tid];
+    const PartOf part = unpack_part(my_part[tid]);
+    for (int i = 0; i < part.parts; ++i)
+      at[i] = make_uint2((columns ? 0x80000000u : 0u) | static_cast<uint32_t>(g * lines + tile),
+                         pack_part(part.slot + i, i, part.parts));
   }
 }
 
@@ -636,6 +676,7 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
   pp.lse_factor = 1.f;
   pp.nbq = static_cast<int>((q->S + block_m - 1) / block_m);
   pp.nbk = static_cast<int>((k->S + block_n - 1) / block_n);
+  pp.bm = block_m, pp.bn = block_n;
   pp.merge_q = merge_of(q->dtype, block_m), pp.merge_k = merge_of(q->dtype, block_n);
   pp.groups_q = (pp.nbq + kGroup - 1) / kGroup, pp.groups_k = (pp.nbk + kGroup - 1) / kGroup;
   pp.row_ptr = row_ptr, pp.col_idx = col_idx, pp.col_capacity = col_capacity;
@@ -646,7 +687,7 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
     pp.lse_factor = kLog2e;
     pp.lse_shift = q->dtype == SAF_F16 ? bwd_f16_p_log2_scale() : 0.f;
     pp.items = 1;
-    SAF_CUDA_TRY(cudaMemsetAsync(pp.w.class_count, 0, (kClasses + 1) * sizeof(int32_t), st));
+    SAF_CUDA_TRY(cudaMemsetAsync(pp.w.class_count, 0, kCounters * sizeof(int32_t), st));
     rc = q->dtype == SAF_BF16 ? launch_prep<__nv_bfloat16>(pp, BH, st) : launch_prep<__half>(pp, BH, st);
     if (rc != SAF_OK) return rc;
     return bsa_bwd_sm100(dout, q, k, v, dq, dk, dv, block_m, block_n, sm_scale, pp.w, st);

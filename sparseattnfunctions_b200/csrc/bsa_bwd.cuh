@@ -30,14 +30,20 @@ struct BwdWorkspace {
   int32_t* count_k;
   // 16-bit kernel only: work items by length (longest class first) and the
   // counters, zeroed before the preparation; the largest |do| of each 128 rows
-  uint32_t* items;       // [kClasses][BH (lines_q + lines_k)]: (1 << 31 for dk / dv) | head * lines + line
+  uint2* items;          // [kClasses][item_cap]: (1 << 31 for dk / dv) | head * lines + line, part (see PartOf)
   int32_t* class_count;  // [kClasses]
   int32_t* next;         // the next item to take
+  int item_cap;
+  // with few heads, long lists are cut into parts whose fp32 sums [128, 64]
+  // (dk or dq, then dv) meet in bwd_merge_kernel; part_cap 0: no list is cut
+  int part_cap;          // parts that fit (16-bit: part is [part_cap][2][128 x 64])
+  int32_t* parts_used;
+  int32_t* split_count;  // lines cut
+  uint2* split;          // [part_cap / 2]: the line as in items, its first part and their number
   float* amax;           // [BH, Sp / 128]
-  // fp32 kernel only, when several CTAs share a tile: their partial sums and
-  // the tiles' counts of finished CTAs
+  float* part;  // partial sums
+  // fp32 kernel only: CTAs that share a tile, and the tiles' counts of finished ones
   int chunks;
-  float* part;
   int* part_count;
   int lines_q, lines_k, cap_q, cap_k;
   int64_t Sp;  // Sq rounded up to 128
@@ -47,5 +53,17 @@ struct BwdWorkspace {
 // Length classes of the work items: class 15 - floor(log2(blocks)), so that
 // the longest lists start first and the short ones fill the last wave.
 constexpr int kClasses = 16;
+
+// Second word of an item: place in `part` | number of the part << 16 | parts << 24
+// (1 part: the line is whole).
+struct PartOf {
+  int slot, number, parts;
+};
+__host__ __device__ inline uint32_t pack_part(int slot, int number, int parts) {
+  return static_cast<uint32_t>(slot) | static_cast<uint32_t>(number) << 16 | static_cast<uint32_t>(parts) << 24;
+}
+__host__ __device__ inline PartOf unpack_part(uint32_t x) {
+  return PartOf{static_cast<int>(x & 0xffffu), static_cast<int>(x >> 16 & 0xffu), static_cast<int>(x >> 24)};
+}
 
 }  // namespace saf

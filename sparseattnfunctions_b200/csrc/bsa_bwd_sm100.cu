@@ -62,7 +62,8 @@ struct Item {
   int32_t g, tile;
   int32_t n;     // walked tiles
   float ds_scale;
-  int32_t pad[3];
+  int32_t part;  // -1, or where the fp32 sums of this part of a line go
+  int32_t pad[2];
 };
 
 struct BwdParams {
@@ -257,7 +258,9 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
   mbar_arrive(c.written());
 }
 
-template <bool kBF16>
+// kParts: lines may be cut into parts (a template, so that the code of the
+// parts costs the launches without them nothing).
+template <bool kBF16, bool kParts>
 __global__ void __launch_bounds__(kThreads, 1)
     bsa_bwd_sm100_kernel(const __grid_constant__ Maps maps, const __grid_constant__ BwdParams p) {
   using L = Layout;
@@ -308,8 +311,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     setmaxnreg_dec<kRegsCtl>();
     if (warp == 0) {
       // ---------------------------------------------------------- producer
-      const int n_items = p.BH * (p.w.lines_q + p.w.lines_k);
       const int mine = lane < kClasses ? p.w.class_count[lane] : 0;  // items per length class
+      int n_items = mine;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) n_items += __shfl_xor_sync(0xffffffffu, n_items, o);
       int it = 0, t = 0, nown = 0, amax_g = -1;
       float ds_scale = 1.f;
       bool ok = true;
@@ -329,7 +334,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         int n = 0, block = kM;
         const uint16_t* list = nullptr;
         if (lin < n_items) {
-          const uint32_t id = p.w.items[static_cast<int64_t>(cls) * n_items + left];
+          const uint2 entry = p.w.items[static_cast<int64_t>(cls) * p.w.item_cap + left];
+          const uint32_t id = entry.x;
+          const PartOf part = unpack_part(entry.y);
+          im.part = kParts && part.parts > 1 ? part.slot : -1;
           im.keys = static_cast<int32_t>(id >> 31);
           const int line = static_cast<int>(id & 0x7fffffffu);
           const int lines = im.keys ? p.w.lines_k : p.w.lines_q;
@@ -340,6 +348,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                          : p.w.list_q + static_cast<int64_t>(line) * p.w.cap_q;
           block = im.keys ? p.bm : p.bn;
           im.n = block == kM ? n : (n + 1) / 2;
+          if (kParts && part.parts > 1) {  // this part's tiles, and their entries of the list
+            const int t0 = im.n * part.number / part.parts, t1 = im.n * (part.number + 1) / part.parts;
+            const int per = kM / block;
+            list += t0 * per;
+            n = min(n - t0 * per, (t1 - t0) * per);
+            im.n = t1 - t0;
+          }
           if (!kBF16 && im.g != amax_g) {
             amax_g = im.g;
             const int chunks = static_cast<int>(p.w.Sp / 128);
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Item im = c.items[slot];
         if (im.keys < 0) break;
         if (!c.wait_all(c.staged(), it & 1)) break;
-        if (lane == 0) {
+        if (lane == 0 && (!kParts || im.part < 0)) {
           const int h = im.g % p.H, b = im.g / p.H;
           const uint32_t src = c.own + slot * 2 * L::kTile;
           for (int x = 0; x < 2; ++x) {
@@ -588,6 +603,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float unscale = kBF16 ? 1.f : 1.f / kF16PScale;
       const float scale = dv ? unscale : kBF16 ? p.scale : p.scale * unscale / ds_scale;
+      const int part = kParts ? c.items[slot].part : -1;
+      if (kParts && part >= 0) {  // sums of a part of the line: fp32, scaled, to the workspace
+        if (keys || (w & 1) == 0) {  // dq: one of the two warpgroups that hold the same 32 channels
+          float* to = p.w.part + (static_cast<int64_t>(part) * 2 + dv) * (kM * kD) + row * kD + (keys ? (w & 1) * 32 : (w >> 1) * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<float4*>(to)[i] =
+                make_float4(__uint_as_float(r[4 * i]) * scale, __uint_as_float(r[4 * i + 1]) * scale,
+                            __uint_as_float(r[4 * i + 2]) * scale, __uint_as_float(r[4 * i + 3]) * scale);
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(c.staged());
+          mbar_arrive(c.own_empty(slot));
+        }
+        ++it;
+        continue;
+      }
       const uint32_t dst = c.own + (2 * slot + (keys && !dv)) * L::kTile + row * 128;
       const int chunk0 = 4 * (keys ? w & 1 : w >> 1);  // 16-byte chunks of the row
 #pragma unroll
@@ -613,16 +646,58 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Adds the parts of a cut line in their order and stores its rows.  One CTA a
+// cut line (the others leave), 8 threads a row of 64 channels; bound by the
+// latency of reading the parts out of L2.
+struct MergeParams {
+  BwdWorkspace w;
+  int H, Sq, Sk;
+  void *dq, *dk, *dv;
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+};
 template <bool kBF16>
+__global__ void __launch_bounds__(256) bwd_merge_kernel(const MergeParams p) {
+  if (static_cast<int>(blockIdx.x) >= *p.w.split_count) return;
+  const uint2 entry = p.w.split[blockIdx.x];
+  const bool keys = entry.x >> 31;
+  const int line = static_cast<int>(entry.x & 0x7fffffffu), lines = keys ? p.w.lines_k : p.w.lines_q;
+  const int g = line / lines, tile = line - g * lines, b = g / p.H, h = g % p.H;
+  const PartOf part = unpack_part(entry.y);
+  const int which = blockIdx.y;  // 0: dk or dq, 1: dv
+  if (which == 1 && !keys) return;
+  const float* src = p.w.part + (static_cast<int64_t>(part.slot) * 2 + which) * (kM * kD);
+  uint8_t* dst = static_cast<uint8_t*>(keys ? (which ? p.dv : p.dk) : p.dq);
+  const int64_t ss = keys ? (which ? p.dv_ss : p.dk_ss) : p.dq_ss;
+  const int64_t at = keys ? (which ? b * p.dv_sb + h * p.dv_sh : b * p.dk_sb + h * p.dk_sh) : b * p.dq_sb + h * p.dq_sh;
+  const int c0 = static_cast<int>(threadIdx.x & 7) * 8;
+  for (int row = threadIdx.x >> 3; row < kM; row += 32) {
+    const int out = tile * kM + row;
+    if (out >= (keys ? p.Sk : p.Sq)) break;
+    float sum[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < part.parts; ++i) {
+      const float4* x = reinterpret_cast<const float4*>(src + static_cast<int64_t>(i) * 2 * (kM * kD) + row * kD + c0);
+      const float4 lo = x[0], hi = x[1];
+      sum[0] += lo.x, sum[1] += lo.y, sum[2] += lo.z, sum[3] += lo.w;
+      sum[4] += hi.x, sum[5] += hi.y, sum[6] += hi.z, sum[7] += hi.w;
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2<kBF16>(pair(sum[2 * i], sum[2 * i + 1]));
+    *reinterpret_cast<uint4*>(dst + 2 * (at + out * ss + c0)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <bool kBF16, bool kParts>
 int32_t launch(const Maps& maps, const BwdParams& p, int grid, cudaStream_t stream) {
-  auto kern = bsa_bwd_sm100_kernel<kBF16>;
+  auto kern = bsa_bwd_sm100_kernel<kBF16, kParts>;
   // a build launched with fewer registers than the split hands out would wait forever
   static const int launch_regs = [] {
     cudaFuncAttributes fa{};
-    return cudaFuncGetAttributes(&fa, bsa_bwd_sm100_kernel<kBF16>) == cudaSuccess ? fa.numRegs : 0;
+    return cudaFuncGetAttributes(&fa, bsa_bwd_sm100_kernel<kBF16, kParts>) == cudaSuccess ? fa.numRegs : 0;
   }();
   if (launch_regs < kLaunchRegs) return SAF_ERR_UNSUPPORTED;
-  if (const int32_t rc = allow_smem<bsa_bwd_sm100_kernel<kBF16>>(Layout::kDynSmem); rc != SAF_OK) return rc;
+  if (const int32_t rc = allow_smem<bsa_bwd_sm100_kernel<kBF16, kParts>>(Layout::kDynSmem); rc != SAF_OK) return rc;
   kern<<<grid, kThreads, Layout::kDynSmem, stream>>>(maps, p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
@@ -658,9 +733,28 @@ int32_t bsa_bwd_sm100(const saf_tensor4* dout, const saf_tensor4* q, const saf_t
   if (p.status == nullptr) return SAF_ERR_CUDA;
   const int sms = current_device_sms();
   if (sms <= 0) return SAF_ERR_CUDA;
-  const int64_t items = static_cast<int64_t>(p.BH) * (w.lines_q + w.lines_k);
-  const int grid = static_cast<int>(items < sms ? items : sms);
-  return q->dtype == SAF_BF16 ? launch<true>(maps, p, grid, stream) : launch<false>(maps, p, grid, stream);
+  const int grid = w.item_cap < sms ? w.item_cap : sms;
+  const bool bf16 = q->dtype == SAF_BF16;
+  if (w.part_cap == 0)
+    return bf16 ? launch<true, false>(maps, p, grid, stream) : launch<false, false>(maps, p, grid, stream);
+  const int32_t rc = bf16 ? launch<true, true>(maps, p, grid, stream) : launch<false, true>(maps, p, grid, stream);
+  if (rc != SAF_OK) return rc;
+  MergeParams m{};
+  m.w = w;
+  m.H = p.H, m.Sq = p.Sq, m.Sk = p.Sk;
+  m.dq = dq->data, m.dk = dk->data, m.dv = dv->data;
+  m.dq_sb = dq->stride_b, m.dq_sh = dq->stride_h, m.dq_ss = dq->stride_s;
+  m.dk_sb = dk->stride_b, m.dk_sh = dk->stride_h, m.dk_ss = dk->stride_s;
+  m.dv_sb = dv->stride_b, m.dv_sh = dv->stride_h, m.dv_ss = dv->stride_s;
+  // a cut line has two parts at least
+  const int64_t lines = static_cast<int64_t>(p.BH) * (w.lines_q + w.lines_k);
+  const dim3 mgrid(static_cast<unsigned>(lines < w.part_cap / 2 ? lines : w.part_cap / 2), 2);
+  if (bf16)
+    bwd_merge_kernel<true><<<mgrid, 256, 0, stream>>>(m);
+  else
+    bwd_merge_kernel<false><<<mgrid, 256, 0, stream>>>(m);
+  SAF_CUDA_TRY(cudaGetLastError());
+  return SAF_OK;
 }
 
 }  // namespace saf

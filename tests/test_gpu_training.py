@@ -412,3 +412,17 @@ def test_autograd_of_sums(cuda_device):
     a.sum().backward()
     ref = kernels.rope(torch.ones_like(a), None, table.cos, table.sin, inverse=True)
     assert torch.equal(q.grad, ref)
+
+
+@pytest.mark.parametrize("dtype,bm,H,Sq,Sk", [(BF16, 128, 1, 5000, 5000), (F16, 64, 1, 3000, 4000), (BF16, 128, 3, 4700, 3900),
+                                              (BF16, 64, 1, 100, 6000)])
+def test_long_lists_of_few_heads(cuda_device, dtype, bm, H, Sq, Sk):
+    """Few heads with dense rows and columns: their lists are cut into parts
+    that are summed afterwards (same tolerances), and give equal bits again."""
+    nbq, nbk = math.ceil(Sq / bm), math.ceil(Sk / bm)
+    mask = _mask(140, 1, H, nbq, nbk, 0.08)
+    mask[..., :2] = True
+    (gq, gk, gv, gd), out, lse, csr, grads = _run(cuda_device, 1, H, Sq, Sk, 64, dtype, bm, bm, 0, seed=141, lead=2, mask=mask)
+    for _ in range(3):
+        again = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)
+        assert all(torch.equal(a, b) for a, b in zip(again, grads))
