@@ -61,7 +61,7 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
   if (q->dtype != SAF_F32) {
     // Cutting pays where one list outlasts an SM's share of the whole.  At
     // 17776 tokens, a tenth of the blocks and dense text, whole and cut lists
-    // take 224 and 98 us at one head, 234 and 137 at two, 235 and 240 at four.
+    // take 232 and 100 us at one head, 245 and 151 at two, 246 and 250 at four.
     const int64_t longest = (q->S > k->S ? q->S : k->S) / 128;
     w.part_cap = BH <= 3 && 2 * longest > 3 * kMinPart ? kPartCap : 0;
     w.item_cap = static_cast<int>(BH * (w.lines_q + w.lines_k)) + w.part_cap;
@@ -89,7 +89,10 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
 }
 
 // ---------------------------------------------------------------------------
-// Preparation: one launch of list blocks and statistics blocks.
+// Preparation: one launch of list blocks and statistics blocks, so that the
+// short chains of the lists hide behind the statistics' reading of out and
+// dout.  Bound by HBM at large sizes (60 heads of 17776 tokens, 16 bits: 273 MB
+// in 62 us, 4.4 TB/s), by a chain of dependent loads at small ones (4 us).
 // ---------------------------------------------------------------------------
 
 struct PrepParams {
@@ -315,7 +318,15 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// CUDA-core gradient.
+// CUDA-core gradient (fp32: the caller wants fp32 accuracy, which TF32 products
+// do not have).  A CTA's two operand pairs lie row-major in shared memory and
+// are read back in both orders; a thread owns 4 x 4 of a 64 x 64 sub-tile.
+// Bound by shared-memory reads and issue (counters: LSU 55 %, issue 60 %): 2
+// heads of 2048 tokens, a quarter of the 64-blocks, take 100 us.  Such
+// sizes have fewer tiles than the GPU takes CTAs, so several CTAs share a
+// tile's walk and the last one to finish adds their sums in a fixed order
+// (163 us unshared, 106 shared; 1, 2, 4, 8 CTAs an SM wanted: 190, 130, 122,
+// 119 us a call).
 // ---------------------------------------------------------------------------
 
 struct SimtBwdParams {

@@ -35,6 +35,37 @@
 // range, so P is formed times 2^4 and dS times a power of two that takes the
 // head's largest |do| to [2^-4, 2^-3); the outputs are scaled back.
 //
+// P and dS are rounded to the 16-bit type because the tensor cores want A and B
+// of one type (walk1 and walk2 are the caller's); the sums over them, S, dP,
+// lse and delta are fp32.  Against sums of unrounded values that makes the
+// error of dk and dv 1.4 times the output's own rounding.  A row of dS sums to
+// zero, so in dq a component that all keys share cancels, but its share of the
+// rounding does not (keys that vary smoothly: 1.5 times the output's rounding,
+// more with a larger common part).  In bf16, dq therefore adds the product of
+// what the rounding took off too, from P's columns, which its items leave free:
+// 1.0 times, and 2.83 instead of 2.61 ms at the size below.  f16 rounds eight
+// times finer and goes without.
+//
+// Bound (2 x 30 heads of 17776 tokens, a tenth of the 128-blocks, bf16): the
+// tensor pipe, the exponentials and the issue slots share the SM, none of them
+// full.  2.79 ms at 1965 MHz = 555 TFLOP/s of the five products that the
+// gradient cannot do without (eight are run: S and dP in both kinds of items,
+// dq in two parts), 3.1 ms once the 1000 W power cap holds the clock at ~1750 MHz.
+// Before dq's second product (2.57 ms), counters at 16 heads: tensor pipe 38 %,
+// MUFU 43 %, issue 41 %, DRAM 10 %, and with a part taken out (2.60 ms a call,
+// timing only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
+// products 2.37, no products at all 1.96, no loads of the walked tiles 2.60,
+// all items empty 0.26.  So the registers' work on a tile (~1400 cycles of a
+// warp) is the longest chain and overlaps with the products only in part.
+//
+// Structures measured against those 2.60 ms and left: two compute warpgroups of
+// 64 columns and one MMA thread 3.60 ms; 64-row units with MMA threads of their
+// own 3.24; two pipelines of 64-row units 2.76; P of all columns before any dS
+// 2.67; a finished item's results read out within the next item 2.89 (spills);
+// exponentials in part on the FMA pipe 2.62 (1/8), 2.65 (1/4), 2.79 (1/2).  One
+// kind of item that adds its share of dq in memory would save two of the
+// products, but wants fp32 atomics, whose order changes the bits from run to run.
+//
 // Every wait is bounded, as in the forward kernel.
 #include "bsa_bwd.cuh"
 
@@ -186,7 +217,6 @@ template <bool kBF16>
 __device__ __forceinline__ uint32_t pack2(f2 x) {
   return kBF16 ? pack_bf16x2(first(x), second(x)) : pack_f16x2(first(x), second(x));
 }
-
 __device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
 #pragma unroll
   for (int e = 0; e < 16; ++e) asm volatile("mov.b32 %0, 0;" : "=r"(r[e]));
@@ -195,10 +225,11 @@ __device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
 // One tile: 32 columns of this thread's row; t is the tile's number in the
 // CTA.  kKeys: lse and delta per column (shared
 // memory; the MMA thread that arrives on `scores` has waited for the stage),
-// and P goes to TMEM too.
+// and P goes to TMEM too.  dq in bf16: the low part of dS takes P's place.
 template <bool kKeys, bool kBF16>
 __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, uint32_t t,
                                              float nl_row, float nd_row, float ds_scale) {
+  constexpr bool kLow = !kKeys && kBF16;
   const uint32_t s = t % kStages, par = t & 1;
   const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t ts = lane_addr + w * kCols;
@@ -234,24 +265,31 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
       f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
       if constexpr (!kBF16) z = mul2(z, mk2(ds_scale, ds_scale));
       dk[e / 2] = pack2<kBF16>(z);
+      if constexpr (kLow) {  // what rounding takes off dS
+        pk[e / 2] = pack2<kBF16>(pair(first(z) - __uint_as_float(dk[e / 2] << 16),
+                                      second(z) - __uint_as_float(dk[e / 2] & 0xffff0000u)));
+      }
     }
   }
   if (!((ent.y >> (quarter >> 1)) & 1)) {  // not listed for this half of the own tile, or no second unit
     zero16(dk);
-    if constexpr (kKeys) zero16(pk);
+    if constexpr (kKeys || kLow) zero16(pk);
   }
   if constexpr (!kKeys) {
     // keys past the end: their scores are 0, not -inf
     const int valid = p.Sk - (ent.x + (w & 1) * kCols);
     if (valid < kCols) {
 #pragma unroll
-      for (int e = 0; e < kCols / 2; ++e)
-        dk[e] = 2 * e + 1 < valid ? dk[e] : 2 * e < valid ? dk[e] & 0xffffu : 0u;
+      for (int e = 0; e < kCols / 2; ++e) {
+        const uint32_t live = 2 * e + 1 < valid ? 0xffffffffu : 2 * e < valid ? 0xffffu : 0u;
+        dk[e] &= live;
+        if constexpr (kLow) pk[e] &= live;
+      }
     }
   }
   pass(c, c.added(), par ^ 1);  // the tile before is multiplied
   tc_fence_after();
-  if constexpr (kKeys) tmem_st16(tp + kColP, pk);
+  if constexpr (kKeys || kLow) tmem_st16(tp + kColP, pk);
   tmem_st16(tp + kColDS, dk);
   tmem_wait_st();
   tc_fence_before();
@@ -519,8 +557,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             const bool both = c.ents[2 * s + 1].y != 0;
-            if (keys) add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
-            add(kColK, kColDS, b, both, j > 0);
+            if (keys) {
+              add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
+              add(kColK, kColDS, b, both, j > 0);
+            } else {
+              if (kBF16) add(kColK, kColP, b, both, j > 0);  // what rounding took off dS
+              add(kColK, kColDS, b, both, kBF16 || j > 0);
+            }
             tc_commit(c.added());
             tc_commit(c.empty(s));
           }

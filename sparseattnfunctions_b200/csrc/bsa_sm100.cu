@@ -303,6 +303,9 @@ constexpr int kMaskKeys = 3;
 constexpr int kMaskPool = 4;
 // Training forward (no mask besides the ragged tail): the row log-sum-exp is
 // stored too, and a row without a live key gives zeros and -inf instead of NaN.
+// 0.88 ms at 2 x 30 heads of 17776 tokens, a tenth of the 128-blocks (0.620
+// TFLOP, 0.43 of the bf16 peak): bound as the mode without a mask, by the
+// exponentials and the hand-overs around them.
 constexpr int kMaskTrain = 5;
 
 // TMA gather4: four rows (coordinates r0..r3 of a 2-D map whose box is one

@@ -12,6 +12,9 @@
 // up to kPlanes heads of q or of k with it: cos and sin are loaded once for
 // them, the heads' loads are all in flight before the first store (so a tensor
 // may be rotated in place), and a head costs one pointer addition.
+// Measured with 1, 2, 4, 8 heads a thread: 60 heads of 17776 tokens, D = 64,
+// bf16, interleaved 118, 84.1, 84.6, 86.3 us (4: 6.5 TB/s, the copy's rate);
+// a long strided half layout in f16 174, 133, 119, 133 us.
 #include "saf_common.cuh"
 
 #include <cuda_bf16.h>

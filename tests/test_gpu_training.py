@@ -426,3 +426,23 @@ def test_long_lists_of_few_heads(cuda_device, dtype, bm, H, Sq, Sk):
     for _ in range(3):
         again = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)
         assert all(torch.equal(a, b) for a, b in zip(again, grads))
+
+
+@pytest.mark.parametrize("H,Sq,Sk,bm,bn", [(2, 300, 700, 64, 64), (2, 500, 333, 128, 128), (1, 200, 5000, 64, 128)])
+def test_keys_with_a_common_part(cuda_device, H, Sq, Sk, bm, bn):
+    """bf16 keys that share a component eight times their spread.  The rows of
+    ds sum to nearly zero, so dq hardly sees it, but a rounding of ds alone
+    would show eight times over (3 U).  A value rounded to nearest is off by
+    2 U / sqrt(12) of its power of two in the mean square, 0.577 U of itself at
+    most; 0.02 U for fp32's part (2e-6 of p, eight times over, and the sums)."""
+    q, k, v, dout = (_randn(150 + i, 1, H, s, 64, dtype=F32) for i, s in enumerate((Sq, Sk, Sk, Sq)))
+    q, k, v, dout = q.to(BF16), (k + 8.0).to(BF16), v.to(BF16), dout.to(BF16)
+    mask = _mask(154, 1, H, math.ceil(Sq / bm), math.ceil(Sk / bn), 0.5)
+    csr = kernels.mask_to_csr(mask.to(cuda_device), bm, bn)
+    gq, gk, gv, gd = (t.to(cuda_device) for t in (q, k, v, dout))
+    out, lse = kernels.bsa_fwd_lse(gq, gk, gv, csr, 0.125)
+    dq = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)[0]
+    live = otr.token_mask(mask, Sq, Sk, bm, bn)
+    ref = otr.attention_grad(dout, q, k, v, out.cpu(), lse.cpu(), live, 0.125)["dq"][0]
+    off = np.linalg.norm(dq.double().cpu().numpy() - ref) / np.linalg.norm(ref)
+    assert off <= 0.6 * U[BF16], f"{off / U[BF16]:.3f} U"
