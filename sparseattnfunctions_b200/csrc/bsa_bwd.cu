@@ -324,9 +324,10 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
 // Bound by shared-memory reads and issue (counters: LSU 55 %, issue 60 %): 2
 // heads of 2048 tokens, a quarter of the 64-blocks, take 100 us.  Such
 // sizes have fewer tiles than the GPU takes CTAs, so several CTAs share a
-// tile's walk and the last one to finish adds their sums in a fixed order
-// (163 us unshared, 106 shared; 1, 2, 4, 8 CTAs an SM wanted: 190, 130, 122,
-// 119 us a call).
+// tile's walk and the last one to finish adds their sums in a fixed order.
+// Larger sizes run the seven products at 26 to 30 TFLOP/s of 72 (16 heads of
+// 4096 tokens 2.4 ms); tiles of 8 x 4 a thread and half the threads left that
+// as it is (2.36 ms) and cost the small sizes 10 %.
 // ---------------------------------------------------------------------------
 
 struct SimtBwdParams {
@@ -386,11 +387,14 @@ template <int D>
 constexpr int kSimtSmem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
 
 // CTAs that share a tile's walk, sub-tile by sub-tile in turn: with few tiles
-// one CTA a tile leaves the GPU idle behind the longest list.  Enough for four
-// CTAs an SM, at most 8; from 592 tiles on there is no split.  (Two heads of
-// 32 tiles each way at 2048 tokens: 200 us unsplit.)
+// one CTA a tile leaves the GPU idle behind the longest list.  Enough for eight
+// CTAs an SM, at most 8; from 1184 tiles on there is no split.  Unsplit, two
+// heads of 32 tiles each way at 2048 tokens took 200 us.  With enough for 4, 8,
+// 12 an SM (at most 16): those and a dense column 146, 139, 145 us, eight heads
+// 424, 378, 376, four heads of 4096 tokens in 128-blocks 727, 625, 592; all of
+// 2 x 1000 tokens 108, 109, 128.
 int simt_chunks(int64_t tiles) {
-  const int64_t want = (4 * 148 + tiles - 1) / tiles;
+  const int64_t want = (8 * 148 + tiles - 1) / tiles;
   return static_cast<int>(want < 1 ? 1 : want > 8 ? 8 : want);
 }
 

@@ -313,8 +313,9 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
 
 // CTAs a 64-row tile of the training forward: four tiles' worth of CTAs an SM,
 // at most 8 a tile (64 tiles of 8 key blocks at 2048 tokens: 90 us unsplit, 71
-// split; 39 with row-major tiles and batched loads).  Bound by shared-memory
-// reads, as the products of a 64 x 64 sub-tile are.
+// split; 39 with row-major tiles and batched loads).  With at most 16 a tile
+// they take 54; with eight an SM, 8 heads of 2048 tokens 124 instead of 131 us,
+// but 16 heads of 4096, D = 128, 1692 instead of 1646.
 int simt_chunks(int64_t tiles) {
   const int64_t want = (4 * 148 + tiles - 1) / tiles;
   return static_cast<int>(want < 1 ? 1 : want > kMaxChunks ? kMaxChunks : want);
