@@ -263,7 +263,7 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
       const f2 pr = pair(ex2_approx(first(y)), ex2_approx(second(y)));
       if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(pr);
       f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
-      if constexpr (!kBF16) z = mul2(z, mk2(ds_scale, ds_scale));
+      if constexpr (!kBF16 && kKeys) z = mul2(z, mk2(ds_scale, ds_scale));
       dk[e / 2] = pack2<kBF16>(z);
       if constexpr (kLow) {  // what rounding takes off dS
         pk[e / 2] = pack2<kBF16>(pair(first(z) - __uint_as_float(dk[e / 2] << 16),
@@ -623,8 +623,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < n; ++j, ++t) compute_tile<true, kBF16>(c, p, w, quarter, t, 0.f, 0.f, ds_scale);
       } else {
         const int64_t at = c.items[slot].g * p.w.Sp + c.items[slot].tile * kM + row;
-        const float nl = p.w.stat_lse[at], nd = p.w.stat_delta[at];
-        for (int j = 0; j < n; ++j, ++t) compute_tile<false, kBF16>(c, p, w, quarter, t, nl, nd, ds_scale);
+        // dS's power of two goes into the exponent: dq does not need P itself
+        const float nl = p.w.stat_lse[at] + (kBF16 ? 0.f : static_cast<float>(ilogbf(ds_scale)));
+        const float nd = p.w.stat_delta[at];
+        for (int j = 0; j < n; ++j, ++t) compute_tile<false, kBF16>(c, p, w, quarter, t, nl, nd, 1.f);
       }
       if (__any_sync(0xffffffffu, *c.abort_flag)) break;
       // Results: warpgroups 0 and 1 take dv, 2 and 3 dk (32 channels each);
