@@ -18,6 +18,8 @@ Modules
                 (utils/merge_unmerge.py:34-154).
   ulysses    -- the pack / unpack layout of the sequence <-> head
                 all-to-all (no reference counterpart: single-GPU reference).
+  training   -- attention with its log-sum-exp, attention's gradient and the
+                rotation, as their formulas (no reference counterpart).
 
 Pinning: ``tests/golden/make_golden.py`` imports the reference from its
 source tree (only where that tree exists, i.e. not on the GPU box) and

@@ -5,6 +5,8 @@ Layout
   build.py              nvcc build of libsaf.so (in-tree)
   _lib.py               ctypes binding, status -> exception mapping
   kernels.py            torch-facing wrappers (pool_topk, mask_to_csr, bsa_fwd, ...)
+  rope.py               rotary tables (3-D video grids, scaled for long contexts)
+  training.py           autograd: rotary positions, block-sparse attention
   geometry.py           CogVideoX token geometry (text + t x h x w video grid)
   workloads.py          seeded synthetic inputs for the benchmark configurations
   special_attentions/   drop-in mirror of the reference package's public API

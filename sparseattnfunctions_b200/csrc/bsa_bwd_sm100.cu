@@ -44,16 +44,16 @@
 // more with a larger common part).  In bf16, dq therefore adds the product of
 // what the rounding took off too, from P's columns, which its items leave free:
 // 1.0 times, and 2.83 instead of 2.61 ms at the size below.  f16 rounds eight
-// times finer and goes without.
+// times finer and goes without (4 heads of 33976 tokens, strided: 0.66 ms a call).
 //
 // Bound (2 x 30 heads of 17776 tokens, a tenth of the 128-blocks, bf16): the
 // tensor pipe, the exponentials and the issue slots share the SM, none of them
 // full.  2.79 ms at 1965 MHz = 555 TFLOP/s of the five products that the
 // gradient cannot do without (eight are run: S and dP in both kinds of items,
 // dq in two parts), 3.1 ms once the 1000 W power cap holds the clock at ~1750 MHz.
-// Before dq's second product (2.57 ms), counters at 16 heads: tensor pipe 38 %,
-// MUFU 43 %, issue 41 %, DRAM 10 %, and with a part taken out (2.60 ms a call,
-// timing only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
+// Counters at 16 heads: tensor pipe 39 %, MUFU 40 %, issue 45 %, DRAM 8 %.
+// Before dq's second product, with a part taken out (2.60 ms whole, timing
+// only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
 // products 2.37, no products at all 1.96, no loads of the walked tiles 2.60,
 // all items empty 0.26.  So the registers' work on a tile (~1400 cycles of a
 // warp) is the longest chain and overlaps with the products only in part.
