@@ -114,7 +114,7 @@ struct PrepParams {
 };
 
 // The lists of 32 mask rows or columns of head g: a bitmap of the live blocks
-// of each line, filled by one thread per listed entry and read back ascending.
+// of each line, filled from the listed entries and read back ascending.
 // A line with an entry outside the mask sets the bad-index flag and skips it.
 __device__ void build_lists(const PrepParams& p, int g, int group, bool columns) {
   extern __shared__ uint32_t sm[];
@@ -135,22 +135,30 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
     rp[i] = x < 0 ? 0 : (static_cast<int64_t>(x) > p.col_capacity ? static_cast<int32_t>(p.col_capacity) : x);
   }
   __syncthreads();
-  for (int e = rp[0] + tid; e < rp[rows]; e += blockDim.x) {
-    int lo = 0, hi = rows;  // the row whose range holds entry e
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (rp[mid] <= e)
-        lo = mid;
-      else
-        hi = mid;
+  // a warp takes four rows at a time, a lane every 32nd entry of each
+  for (int r0 = warp * 4; r0 < rows; r0 += 32) {
+    int at[4], end[4], most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      at[i] = r0 + i < rows ? rp[r0 + i] : 0;
+      end[i] = r0 + i < rows ? rp[r0 + i + 1] : 0;
+      most = max(most, end[i] - at[i]);
     }
-    const int c = p.col_idx[e];
-    if (c < 0 || c >= p.nbk) {
-      atomicOr(p.status, SAF_DEV_BADINDEX);
-      continue;
+    for (int k = lane; k - lane < most; k += 32) {
+      int c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = k < end[i] - at[i] ? p.col_idx[at[i] + k] : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k >= end[i] - at[i]) continue;
+        if (c[i] < 0 || c[i] >= p.nbk) {
+          atomicOr(p.status, SAF_DEV_BADINDEX);
+          continue;
+        }
+        const int line = columns ? c[i] - line0 : r0 + i, bit = columns ? row0 + r0 + i : c[i];
+        if (line >= 0 && line < kGroup) atomicOr(&bits[line * words + (bit >> 5)], 1u << (bit & 31));
+      }
     }
-    const int line = columns ? c - line0 : lo, bit = columns ? row0 + lo : c;
-    if (line >= 0 && line < kGroup) atomicOr(&bits[line * words + (bit >> 5)], 1u << (bit & 31));
   }
   __syncthreads();
   const int merge = columns ? p.merge_k : p.merge_q;
@@ -194,7 +202,7 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
         if (p.w.part_cap > 0) {
           const int64_t entries = p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1) + p.nbq] -
                                   p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1)];
-          const int64_t work = 2 * entries * (p.bm * p.bn) / (128 * 128) * gridDim.y;
+          const int64_t work = 2 * entries * (p.bm * p.bn) / (128 * 128) * gridDim.x;
           const int64_t share = max(static_cast<int64_t>(kMinPart), (work + 147) / 148);
           if (2 * static_cast<int64_t>(tiles) > 3 * share) {
             parts = static_cast<int>(min(static_cast<int64_t>(kMaxParts), (tiles + share - 1) / share));
@@ -253,21 +261,26 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   if constexpr (sizeof(T) == 2) {  // D = 64: 8 lanes of 16 bytes a row
     const int sub = lane & 7;
     float amax = 0.f;
+    constexpr int kRows = kRowChunk / 32;  // a thread's rows, all in flight
+    uint4 x[kRows], y[kRows];
 #pragma unroll
-    for (int i = 0; i < kRowChunk / 32; ++i) {
+    for (int i = 0; i < kRows; ++i) {
+      const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
+      const bool in = row < p.Sq;
+      x[i] = in ? *reinterpret_cast<const uint4*>(o + row * p.o_ss + sub * 8) : uint4{0, 0, 0, 0};
+      y[i] = in ? *reinterpret_cast<const uint4*>(d + row * p.d_ss + sub * 8) : uint4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
       const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
       float sum = 0.f;
-      if (row < p.Sq) {
-        const uint4 x = *reinterpret_cast<const uint4*>(o + row * p.o_ss + sub * 8);
-        const uint4 y = *reinterpret_cast<const uint4*>(d + row * p.d_ss + sub * 8);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 fx = unpack2(xs[e], static_cast<const T*>(nullptr));
-          const float2 fy = unpack2(ys[e], static_cast<const T*>(nullptr));
-          sum = fmaf(fx.x, fy.x, fmaf(fx.y, fy.y, sum));
-          amax = fmaxf(amax, fmaxf(fabsf(fy.x), fabsf(fy.y)));
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float2 fx = unpack2(xs[e], static_cast<const T*>(nullptr));
+        const float2 fy = unpack2(ys[e], static_cast<const T*>(nullptr));
+        sum = fmaf(fx.x, fy.x, fmaf(fx.y, fy.y, sum));
+        amax = fmaxf(amax, fmaxf(fabsf(fy.x), fabsf(fy.y)));
       }
 #pragma unroll
       for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -308,7 +321,7 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
 
 template <typename T>
 __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
-  const int g = blockIdx.y, x = blockIdx.x;
+  const int g = blockIdx.x, x = blockIdx.y;  // every head's lists start before the statistics
   if (x < p.groups_k)
     build_lists(p, g, x, true);
   else if (x < p.groups_k + p.groups_q)
@@ -618,7 +631,7 @@ int32_t launch_prep(const PrepParams& p, int BH, cudaStream_t st) {
   const int smem = (kGroup * words + rows + 1) * 4;
   if (smem > 48 * 1024)
     if (const int32_t rc = allow_smem<bwd_prep_kernel<T>>(smem); rc != SAF_OK) return rc;
-  const dim3 grid(static_cast<unsigned>(p.groups_k + p.groups_q + p.w.Sp / kRowChunk), static_cast<unsigned>(BH));
+  const dim3 grid(static_cast<unsigned>(BH), static_cast<unsigned>(p.groups_k + p.groups_q + p.w.Sp / kRowChunk));
   bwd_prep_kernel<T><<<grid, 256, smem, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
