@@ -66,10 +66,12 @@ def _t4(x: torch.Tensor) -> _lib.Tensor4:
 _PACK_T4 = struct.Struct("Pii7q").pack  # saf_tensor4
 
 
-def _p4(x: torch.Tensor) -> bytes:
-    """saf_tensor4 of a [B, H, S, D] tensor with a contiguous D, packed (half
-    the cost of a ctypes structure; ctypes passes the bytes by address)."""
-    return _PACK_T4(x.data_ptr(), _DTYPES[x.dtype], 0, *x.shape, *x.stride()[:3])
+def _p4(x: torch.Tensor, B: int, H: int, S: int, D: int) -> bytes:
+    """saf_tensor4 of a tensor of the (checked) shape [B, H, S, D] with a
+    contiguous D, packed (a third of the cost of a ctypes structure; ctypes
+    passes the bytes by address).  The library refuses a type it lacks."""
+    sb, sh, ss, _ = x.stride()
+    return _PACK_T4(x.data_ptr(), _DTYPES.get(x.dtype, -1), 0, B, H, S, D, sb, sh, ss)
 
 
 def _d_last(x: torch.Tensor) -> torch.Tensor:
@@ -406,20 +408,20 @@ def bsa_fwd_pool(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCS
     return out, pool
 
 
-def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     qs, ks = q.shape, k.shape
-    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[:2] != qs[:2] or ks[3] != qs[3]:
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[1] != qs[1] or ks[3] != qs[3]:
         raise ValueError(f"q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} do not match")
+    return (*qs, ks[2])
 
 
-def _check_csr(csr: BlockCSR, q: torch.Tensor, k: torch.Tensor) -> None:
-    B, H, Sq, _ = q.shape
-    if (csr.B, csr.H) != (B, H) or csr.nbq != math.ceil(Sq / csr.block_m) or \
-            csr.nbk != math.ceil(k.shape[2] / csr.block_n):
+def _check_csr(csr: BlockCSR, B: int, H: int, Sq: int, Sk: int) -> None:
+    nbq = csr.nbq
+    if csr.B != B or csr.H != H or nbq != -(-Sq // csr.block_m) or csr.nbk != -(-Sk // csr.block_n):
         raise ValueError("block list does not match q/k shapes")
-    if csr.row_ptr.dtype != torch.int32 or csr.col_idx.dtype != torch.int32 or \
-            csr.row_ptr.numel() != B * H * (csr.nbq + 1) or \
-            not (csr.row_ptr.is_contiguous() and csr.col_idx.is_contiguous()):
+    row_ptr, col_idx = csr.row_ptr, csr.col_idx
+    if row_ptr.dtype != torch.int32 or col_idx.dtype != torch.int32 or row_ptr.numel() != B * H * (nbq + 1) or \
+            not (row_ptr.is_contiguous() and col_idx.is_contiguous()):
         raise ValueError("block list must hold contiguous int32 row_ptr [B*H, nbq + 1] and col_idx")
 
 
@@ -428,9 +430,10 @@ def _rows_last(x: torch.Tensor, unit: int) -> torch.Tensor:
     ``unit`` elements: a gradient comes in whatever layout the code after an
     operator left it (expanded, an odd offset), which the caller does not
     choose."""
-    if x.dim() == 4 and (x.stride(3) != 1 or x.stride(2) < x.shape[3] or x.data_ptr() % (unit * x.element_size())
-                         or any(s % unit for s in x.stride()[:3])):
-        return x.clone(memory_format=torch.contiguous_format)
+    if x.dim() == 4:
+        sb, sh, ss, sd = x.stride()
+        if sd != 1 or ss < x.shape[3] or x.data_ptr() % (unit * x.element_size()) or sb % unit or sh % unit or ss % unit:
+            return x.clone(memory_format=torch.contiguous_format)
     return x
 
 
@@ -442,22 +445,22 @@ def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR
     key gives zeros and ``-inf`` (``bsa_fwd`` gives NaN there)."""
     dev = _device_of(q, k, v, csr.row_ptr, csr.col_idx)
     q, k, v = _d_last(q), _d_last(k), _d_last(v)
-    _check_qkv(q, k, v)
-    _check_csr(csr, q, k)
+    B, H, Sq, D, Sk = _check_qkv(q, k, v)
+    _check_csr(csr, B, H, Sq, Sk)
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have the shape, type and device of q")
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    lse = q.new_empty((B, H, Sq), dtype=torch.float32)
     if q.numel() == 0 or k.numel() == 0:  # no key at all is a row without a live key
         return out.zero_(), lse.fill_(-math.inf)
     lib = _lib.load()
-    tq, tk, tv, to = _p4(q), _p4(k), _p4(v), _p4(out)
+    tq, tk, tv, to = _p4(q, B, H, Sq, D), _p4(k, B, H, Sk, D), _p4(v, B, H, Sk, D), _p4(out, B, H, Sq, D)
     lead, ws_bytes, ws_ptr = int(csr.dense_rows), 0, None
     if lead > 0 or q.dtype == torch.float32:
         ws_bytes = lib.saf_bsa_fwd_lse_workspace_bytes(tq, tk, csr.block_m, lead)
         if ws_bytes:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            ws = q.new_empty(ws_bytes, dtype=torch.uint8)
             ws_ptr = ws.data_ptr()
     rc = lib.saf_bsa_fwd_lse(tq, tk, tv, to, csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(),
                              csr.block_m, csr.block_n, sm_scale, lead, lse.data_ptr(), ws_ptr, ws_bytes,
@@ -477,26 +480,28 @@ def bsa_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     dev = _device_of(dout, q, k, v, out, lse, csr.row_ptr, csr.col_idx)
     dout = _rows_last(dout, 1 if dout.dtype == torch.float32 else 8)
     q, k, v, out = _d_last(q), _d_last(k), _d_last(v), _d_last(out)
-    _check_qkv(q, k, v)
-    _check_csr(csr, q, k)
+    B, H, Sq, D, Sk = _check_qkv(q, k, v)
+    _check_csr(csr, B, H, Sq, Sk)
     if dout.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"dout {tuple(dout.shape)} and out {tuple(out.shape)} must match q {tuple(q.shape)}")
-    if lse.dtype != torch.float32 or lse.shape != q.shape[:3]:
-        raise ValueError(f"lse must be a float32 {list(q.shape[:3])} tensor")
+    if lse.dtype != torch.float32 or lse.shape != (B, H, Sq):
+        raise ValueError(f"lse must be a float32 {[B, H, Sq]} tensor")
     lb, lh, ls = lse.stride()
-    if ls != 1 or lh < lse.shape[2] or lb != lse.shape[1] * lh:
+    if ls != 1 or lh < Sq or lb != H * lh:
         lse = lse.contiguous()
         lh = lse.stride(1)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     lib = _lib.load()
-    tq, tk = _p4(q), _p4(k)
-    ws_bytes = lib.saf_bsa_bwd_workspace_bytes(tq, tk, csr.block_m, csr.block_n)
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-    rc = lib.saf_bsa_bwd(_p4(dout), tq, tk, _p4(v), _p4(out), lse.data_ptr(), lh, _p4(dq), _p4(dk), _p4(dv),
-                         csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(), csr.block_m,
-                         csr.block_n, sm_scale, ws.data_ptr(), ws_bytes, _stream_ptr(dev))
+    block_m, block_n, row_ptr, col_idx = csr.block_m, csr.block_n, csr.row_ptr, csr.col_idx
+    tq, tk = _p4(q, B, H, Sq, D), _p4(k, B, H, Sk, D)
+    ws_bytes = lib.saf_bsa_bwd_workspace_bytes(tq, tk, block_m, block_n)
+    ws = q.new_empty(max(ws_bytes, 16), dtype=torch.uint8)
+    rc = lib.saf_bsa_bwd(_p4(dout, B, H, Sq, D), tq, tk, _p4(v, B, H, Sk, D), _p4(out, B, H, Sq, D), lse.data_ptr(),
+                         lh, _p4(dq, B, H, Sq, D), _p4(dk, B, H, Sk, D), _p4(dv, B, H, Sk, D), row_ptr.data_ptr(),
+                         col_idx.data_ptr(), col_idx.numel(), block_m, block_n, sm_scale, ws.data_ptr(), ws_bytes,
+                         _stream_ptr(dev))
     if rc:
         _lib.check("saf_bsa_bwd", rc)
     return dq, dk, dv
@@ -523,7 +528,7 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: tor
     dev = _device_of(q, cos, sin) if k is None else _device_of(q, k, cos, sin)
     if q.dim() != 4:
         raise ValueError(f"q must be a [B, H, S, D] tensor, got shape {tuple(q.shape)}")
-    B, _, S, D = q.shape
+    B, H, S, D = q.shape
     if k is not None and (k.dtype != q.dtype or k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
         raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more than heads")
     text_len = int(text_len)
@@ -549,7 +554,11 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: tor
                 raise ValueError("out must match q (and k) in shape, type and device")
     if q.numel() and (k is None or k.numel()):
         cos, sin = cos.contiguous(), sin.contiguous()
-        rc = _lib.load().saf_rope(_p4(q), None if k is None else _p4(k), _p4(oq), None if k is None else _p4(ok),
+        tk = to = None
+        if k is not None:
+            Hk = k.shape[1]
+            tk, to = _p4(k, B, Hk, S, D), _p4(ok, B, Hk, S, D)
+        rc = _lib.load().saf_rope(_p4(q, B, H, S, D), tk, _p4(oq, B, H, S, D), to,
                                   cos.data_ptr(), sin.data_ptr(), cos.stride(0) if len(table) == 3 else 0, text_len,
                                   R, half, inverse, _stream_ptr(dev))
         if rc:
