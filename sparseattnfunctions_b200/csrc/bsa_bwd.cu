@@ -322,6 +322,8 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
 template <typename T>
 __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
   const int g = blockIdx.x, x = blockIdx.y;  // every head's lists start before the statistics
+  // the 16-bit gradient may set itself up once every block here has started
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (x < p.groups_k)
     build_lists(p, g, x, true);
   else if (x < p.groups_k + p.groups_q)
