@@ -44,13 +44,13 @@
 // more with a larger common part).  In bf16, dq therefore adds the product of
 // what the rounding took off too, from P's columns, which its items leave free:
 // 1.0 times, and 2.83 instead of 2.61 ms at the size below.  f16 rounds eight
-// times finer and goes without (4 heads of 33976 tokens, strided: 0.66 ms a call).
+// times finer and goes without (4 heads of 33976 tokens, strided: 0.61 ms).
 //
 // Bound (2 x 30 heads of 17776 tokens, a tenth of the 128-blocks, bf16): the
 // tensor pipe, the exponentials and the issue slots share the SM, none of them
-// full.  2.79 ms at 1965 MHz = 555 TFLOP/s of the five products that the
+// full.  2.78 ms at 1965 MHz = 558 TFLOP/s of the five products that the
 // gradient cannot do without (eight are run: S and dP in both kinds of items,
-// dq in two parts), 3.1 ms once the 1000 W power cap holds the clock at ~1750 MHz.
+// dq in two parts), 3.1 to 3.2 ms once the 1000 W power cap holds the clock lower.
 // Counters at 16 heads: tensor pipe 39 %, MUFU 40 %, issue 45 %, DRAM 8 %.
 // Before dq's second product, with a part taken out (2.60 ms whole, timing
 // only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
