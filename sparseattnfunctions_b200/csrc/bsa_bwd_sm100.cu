@@ -120,7 +120,7 @@ struct Layout {
   static constexpr int kOffItem = kOffStat + kStages * kStat;
   static constexpr int kOffEnt = kOffItem + 2 * static_cast<int>(sizeof(Item));
   static constexpr int kOffBar = kOffEnt + kStages * 16;
-  static constexpr int kBars = 4 + 2 * kStages + 9;
+  static constexpr int kBars = 4 + 2 * kStages + 10;
   static constexpr int kOffMisc = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffMisc + 16;
   static constexpr int kDynSmem = kBytes + 1024;  // slack for 1024-byte alignment
@@ -162,9 +162,14 @@ struct Ctx {
   __device__ uint32_t added() const { return at(3); }      // and multiplied
   __device__ uint32_t acc_full() const { return at(4); }   // the item's sums are final
   __device__ uint32_t acc_empty() const { return at(5); }  // and read
-  __device__ uint32_t staged() const { return at(6); }     // the results are in shared memory
-  __device__ uint32_t drain(int w) const { return at(7 + w); }
-  __device__ bool wait(uint32_t bar, uint32_t parity) const { 
+  // The results of the item in slot s are in shared memory.  One barrier a
+  // slot: an item without tiles waits for no product, so a compute warp may
+  // arrive for it while another is still at the item before.  It cannot be a
+  // whole round ahead: the slot's next item needs own_empty, which holds every
+  // compute warp and the store warp.
+  __device__ uint32_t staged(int s) const { return at(6 + s); }
+  __device__ uint32_t drain(int w) const { return at(8 + w); }
+  __device__ bool wait(uint32_t bar, uint32_t parity) const {
     return mbar_wait(bar, parity, abort_flag, p.status, p.budget_ns);
   }
   // the 32 lanes of a warp together
@@ -320,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(c.own_full(s), 1);
       mbar_init(c.own_empty(s), 3 + kComputeWarps);  // MMA threads, store warp, compute warps
+      mbar_init(c.staged(s), kComputeWarps);
       mbar_init(c.drain(s), 1);
     }
     for (int s = 0; s < kStages; ++s) {
@@ -332,7 +338,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(c.added(), 1);
     mbar_init(c.acc_full(), 1);
     mbar_init(c.acc_empty(), kComputeWarps);
-    mbar_init(c.staged(), kComputeWarps);
     *c.abort_flag = 0;
     fence_mbar_init();
   }
@@ -583,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!c.wait_all(c.own_full(slot), (it >> 1) & 1)) break;
         const Item im = c.items[slot];
         if (im.keys < 0) break;
-        if (!c.wait_all(c.staged(), it & 1)) break;
+        if (!c.wait_all(c.staged(slot), (it >> 1) & 1)) break;
         if (lane == 0 && (!kParts || im.part < 0)) {
           const int h = im.g % p.H, b = im.g / p.H;
           const uint32_t src = c.own + slot * 2 * L::kTile;
@@ -663,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(c.staged());
+          mbar_arrive(c.staged(slot));
           mbar_arrive(c.own_empty(slot));
         }
         ++it;
@@ -684,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(c.staged());
+        mbar_arrive(c.staged(slot));
         mbar_arrive(c.own_empty(slot));
       }
       ++it;
