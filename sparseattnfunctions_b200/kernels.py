@@ -408,6 +408,15 @@ def bsa_fwd_pool(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCS
     return out, pool
 
 
+def _check_out(out: torch.Tensor, like: torch.Tensor) -> None:
+    """A caller's ``out``: as ``like``, and D contiguous (saf_tensor4 has no
+    stride for D, so the library could not notice)."""
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError("out must match its input in shape, type and device")
+    if out.stride(-1) != 1:
+        raise ValueError("the last (D) dimension of out must be contiguous")
+
+
 def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4 or v.shape != ks or ks[0] != qs[0] or ks[1] != qs[1] or ks[3] != qs[3]:
@@ -449,8 +458,8 @@ def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR
     _check_csr(csr, B, H, Sq, Sk)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError("out must have the shape, type and device of q")
+    else:
+        _check_out(out, q)
     lse = q.new_empty((B, H, Sq), dtype=torch.float32)
     if q.numel() == 0 or k.numel() == 0:  # no key at all is a row without a live key
         return out.zero_(), lse.fill_(-math.inf)
@@ -549,9 +558,9 @@ def rope(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: tor
         oq, ok = (out, None) if isinstance(out, torch.Tensor) else out if len(out) == 2 else (None, None)
         if oq is None or (ok is None) != (k is None):
             raise ValueError("out must hold one tensor for q and one for k")
-        for o, x in ((oq, q),) if k is None else ((oq, q), (ok, k)):
-            if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device:
-                raise ValueError("out must match q (and k) in shape, type and device")
+        _check_out(oq, q)
+        if k is not None:
+            _check_out(ok, k)
     if q.numel() and (k is None or k.numel()):
         cos, sin = cos.contiguous(), sin.contiguous()
         tk = to = None

@@ -45,3 +45,29 @@ def test_empty_lines_between_listed_ones(cuda_device, dtype, bm, bn):
         _fill((gq, gk, gv), 7.0)
         again = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)
         assert all(torch.equal(a, b) for a, b in zip(again, first))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_out_needs_a_contiguous_last_dimension(cuda_device, dtype):
+    """A destination whose channels are apart is refused, not written as if they
+    were side by side; rows that are apart are fine."""
+    q, k = (_randn(210 + i, 1, 2, 200, 64, dtype=dtype).to(cuda_device) for i in range(2))
+    csr = kernels.mask_to_csr(torch.ones(1, 2, 2, 2, dtype=torch.bool, device=cuda_device), 128, 128)
+    table = torch.ones(200, 32, device=cuda_device), torch.zeros(200, 32, device=cuda_device)
+    good = torch.empty_like(q)
+    apart = torch.full((1, 2, 200, 128), 5.0, dtype=dtype, device=cuda_device)
+    turned = torch.full((1, 2, 64, 200), 5.0, dtype=dtype, device=cuda_device)
+    for bad in (apart[..., ::2], turned.transpose(2, 3)):
+        for call in (lambda: kernels.bsa_fwd_lse(q, k, k, csr, 0.125, out=bad),
+                     lambda: kernels.rope(q, k, *table, out=(bad, good)),
+                     lambda: kernels.rope(q, k, *table, out=(good, bad)),
+                     lambda: kernels.rope(q, None, *table, out=bad),
+                     lambda: kernels.rope(bad, k, *table, out=(bad, good))):
+            with pytest.raises(ValueError):
+                call()
+    assert bool((apart == 5).all()) and bool((turned == 5).all())
+    kernels.rope(q, k, *table, out=(apart[..., :64], good))
+    assert torch.equal(apart[..., :64], q) and torch.equal(good, k) and bool((apart[..., 64:] == 5).all())
+    ref = kernels.bsa_fwd_lse(q, k, k, csr, 0.125)[0]
+    kernels.bsa_fwd_lse(q, k, k, csr, 0.125, out=apart[..., 64:])
+    assert torch.equal(apart[..., 64:], ref)
