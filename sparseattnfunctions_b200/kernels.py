@@ -436,12 +436,13 @@ def _check_csr(csr: BlockCSR, B: int, H: int, Sq: int, Sk: int) -> None:
 
 def _rows_last(x: torch.Tensor, unit: int) -> torch.Tensor:
     """``x``, copied unless its rows are whole, apart, and start at multiples of
-    ``unit`` elements: a gradient comes in whatever layout the code after an
-    operator left it (expanded, an odd offset), which the caller does not
-    choose."""
+    ``unit`` elements (above 1 for TMA, which also takes no stride of 0): a
+    gradient comes in whatever layout the code after an operator left it
+    (expanded, an odd offset), which the caller does not choose."""
     if x.dim() == 4:
         sb, sh, ss, sd = x.stride()
-        if sd != 1 or ss < x.shape[3] or x.data_ptr() % (unit * x.element_size()) or sb % unit or sh % unit or ss % unit:
+        if sd != 1 or ss < x.shape[3] or (unit > 1 and not (sb and sh)) or x.data_ptr() % (unit * x.element_size()) or \
+                sb % unit or sh % unit or ss % unit:
             return x.clone(memory_format=torch.contiguous_format)
     return x
 

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from oracle import training as otr
-from sparseattnfunctions_b200 import kernels
+from sparseattnfunctions_b200 import kernels, training
 from test_gpu_training import BF16, F16, U, _check_fwd, _check_grad, _mask, _randn  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,20 @@ def test_out_needs_a_contiguous_last_dimension(cuda_device, dtype):
     ref = kernels.bsa_fwd_lse(q, k, k, csr, 0.125)[0]
     kernels.bsa_fwd_lse(q, k, k, csr, 0.125, out=apart[..., 64:])
     assert torch.equal(apart[..., 64:], ref)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, torch.float32])
+def test_gradient_expanded_over_heads_or_batch(cuda_device, dtype):
+    """What autograd hands over behind a sum over heads or batch rows: a stride
+    of 0 in those dimensions, whole rows inside."""
+    q, k, v, d = (_randn(220 + i, 2, 3, 200, 64, dtype=dtype).to(cuda_device) for i in range(4))
+    csr = kernels.mask_to_csr(torch.ones(2, 3, 2, 2, dtype=torch.bool, device=cuda_device), 128, 128)
+    out, lse = kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+    for dout in (d[:, :1].expand(d.shape), d[:1].expand(d.shape), d[:1, :1].expand(d.shape)):
+        got = kernels.bsa_bwd(dout, q, k, v, out, lse, csr, 0.125)
+        ref = kernels.bsa_bwd(dout.contiguous(), q, k, v, out, lse, csr, 0.125)
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    training.sparse_attention(*x, csr, 0.125).sum(1).mul(d[:, 0]).sum().backward()
+    ref = kernels.bsa_bwd(d[:, :1].expand(d.shape).contiguous(), q, k, v, out, lse, csr, 0.125)
+    assert all(torch.equal(a.grad, b) for a, b in zip(x, ref))
