@@ -203,7 +203,9 @@ int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor
  * Unlike saf_bsa_fwd, a row with no live key gives o = 0 and lse = -inf.
  * sm_scale is positive and finite.  workspace (16-byte aligned, of
  * saf_bsa_fwd_lse_workspace_bytes; 0 bytes: may be null) holds the partial
- * rows of split tiles, so launches may overlap on a device.
+ * rows of split tiles and the launch's counters.  Nothing is shared between
+ * launches: those with a workspace each may overlap on a device, replays of
+ * captured ones too.
  * No counterpart in the reference, whose kernel has no training path
  * (utils/block_sparse_attn_kernel.py:278-281). */
 size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,

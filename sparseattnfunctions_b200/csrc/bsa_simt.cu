@@ -18,7 +18,7 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
                       int64_t bias_stride, float sm_scale, int lead_tiles, const int32_t* row_ranges,
                       const FrameMaskArgs* frames, const PoolArgs* pool, const TrainArgs* train,
                       cudaStream_t stream);
-int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles, int64_t* part_bytes);
+TrainSpace bsa_train_space(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles);
 int32_t bsa_fwd_sm100_keys(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
                            const saf_tensor4* o, const int32_t* key_list, int32_t key_len,
                            const int32_t* key_batch, float sm_scale, cudaStream_t stream);
@@ -485,29 +485,28 @@ extern "C" int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const
                             kv_bias_stride_bh, sm_scale, lead_rows, nullptr, stream);
 }
 
-// Bytes of a training forward's split buffers (0: every tile runs unsplit).
-static int64_t train_ws_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m, int32_t lead_rows,
-                              int64_t* part_bytes);
-
 static int64_t lead_tiles_of(int32_t lead_rows, int32_t block_m) {
   return (static_cast<int64_t>(lead_rows) * block_m + 127) / 128;
+}
+
+// A training forward's buffers: fp32 as bsa_fwd_simt splits its tiles.
+static TrainSpace train_space(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m, int32_t lead_rows) {
+  if (q->dtype != SAF_F32)
+    return bsa_train_space(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m));
+  const int64_t tiles = q->B * q->H * ((q->S + kT - 1) / kT);
+  const int chunks = simt_chunks(tiles);
+  TrainSpace s{};
+  if (chunks > 1) {
+    s.part = tiles * chunks * kT * (q->D + 2) * static_cast<int64_t>(sizeof(float));
+    s.cnt = tiles * static_cast<int64_t>(sizeof(int));
+  }
+  return s;
 }
 
 extern "C" size_t saf_bsa_fwd_lse_workspace_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m,
                                                  int32_t lead_rows) {
   if (check_tensor4(q) != SAF_OK || check_tensor4(k) != SAF_OK || block_m <= 0 || lead_rows < 0) return 0;
-  int64_t part;
-  return static_cast<size_t>(train_ws_bytes(q, k, block_m, lead_rows, &part));
-}
-
-static int64_t train_ws_bytes(const saf_tensor4* q, const saf_tensor4* k, int32_t block_m, int32_t lead_rows,
-                              int64_t* part_bytes) {
-  if (q->dtype != SAF_F32)
-    return bsa_train_split_bytes(q->B * q->H, q->S, k->S, lead_tiles_of(lead_rows, block_m), part_bytes);
-  const int64_t tiles = q->B * q->H * ((q->S + kT - 1) / kT);
-  const int chunks = simt_chunks(tiles);
-  *part_bytes = chunks > 1 ? tiles * chunks * kT * (q->D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
-  return chunks > 1 ? *part_bytes + tiles * static_cast<int64_t>(sizeof(int)) : 0;
+  return static_cast<size_t>(train_space(q, k, block_m, lead_rows).bytes());
 }
 
 extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor4* v,
@@ -521,14 +520,18 @@ extern "C" int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, c
   if (block_m <= 0 || lead_rows < 0) return SAF_ERR_ARG;
   for (const saf_tensor4* t : {k, v, o})
     if ((rc = check_operand(t, q)) != SAF_OK) return rc;
-  TrainArgs train{lse, nullptr, nullptr};
-  int64_t part = 0;
-  const int64_t need = train_ws_bytes(q, k, block_m, lead_rows, &part);
-  if (need > 0) {
-    if (workspace == nullptr || workspace_bytes < static_cast<size_t>(need)) return SAF_ERR_WORKSPACE;
+  TrainArgs train{};
+  train.lse = lse;
+  const TrainSpace space = train_space(q, k, block_m, lead_rows);
+  if (space.bytes() > 0) {
+    if (workspace == nullptr || workspace_bytes < static_cast<size_t>(space.bytes())) return SAF_ERR_WORKSPACE;
     if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return SAF_ERR_STRIDE;
-    train.split_part = static_cast<float*>(workspace);
-    train.split_cnt = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + part);
+    uint8_t* at = static_cast<uint8_t*>(workspace);
+    if (space.part > 0) {
+      train.split_part = reinterpret_cast<float*>(at);
+      train.split_cnt = reinterpret_cast<int*>(at + space.part);
+    }
+    if (space.tile > 0) train.tile_ctr = reinterpret_cast<unsigned int*>(at + space.part + space.cnt);
   }
   return bsa_fwd_entry(q, k, v, o, row_ptr, col_idx, col_capacity, block_m, block_n, nullptr, 0,
                        sm_scale, lead_rows, nullptr, nullptr, nullptr, &train, stream);

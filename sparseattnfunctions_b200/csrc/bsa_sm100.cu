@@ -112,7 +112,9 @@ struct BsaParams {
   int pool_block, nbp;
   float* lse;  // training mode: natural log-sum-exp of every row, [B*H, Sq]
   // persistent schedule: query tiles per head, heads, and this launch's
-  // [next tile, CTAs done] counters (zero on entry; the last CTA resets them)
+  // [next tile, CTAs done] counters (zero on entry; the last CTA resets them).
+  // Training mode: the next tile alone, in the caller's workspace; null when
+  // there is a CTA for every item
   int n_tiles, BH;
   unsigned int* tile_ctr;
   int list_cap;  // entries of a tile's block list in shared memory (nbk rounded up to 8)
@@ -475,7 +477,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     while (ok) {
       // next tile: fetched by lane 0, published in ring slot ti & 1
       int lin = 0;
-      if (lane == 0) lin = static_cast<int>(atomicAdd(p.tile_ctr, 1u));
+      if constexpr (kMask == kMaskTrain) {  // the first item without the counter
+        if (ti == 0)
+          lin = blockIdx.x;
+        else if (p.tile_ctr == nullptr)
+          lin = n_total;
+        else if (lane == 0)
+          lin = static_cast<int>(gridDim.x + atomicAdd(p.tile_ctr, 1u));
+      } else if (lane == 0) {
+        lin = static_cast<int>(atomicAdd(p.tile_ctr, 1u));
+      }
       lin = __shfl_sync(0xffffffffu, lin, 0);
       const int slot = ti & 1;
       ok = mbar_wait(bar_tile_empty(slot), ((ti >> 1) & 1) ^ 1, abort_flag, p.status, p.budget_ns);
@@ -1179,7 +1190,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     named_barrier_sync(1, kThreads);
   }
   // The last CTA to finish resets this launch's tile counters.
-  if (threadIdx.x == 0) {
+  if (kMask != kMaskTrain && threadIdx.x == 0) {
     __threadfence();
     if (atomicAdd(p.tile_ctr + 1, 1u) == gridDim.x - 1) {
       p.tile_ctr[0] = 0u;
@@ -1254,6 +1265,10 @@ int split_cap(int64_t items, int sms) {
 // clearing and the merge), 33 blocks 47.2 and 35.0, 139 blocks 181 and 60.
 int train_split_cap(int64_t items, int64_t Sk) { return Sk > 24 * 128 ? split_cap(items, kTrainSms) : 1; }
 
+// Up to two items an SM the training forward gives each item a CTA of its own
+// and needs no counter (nor its clearing).
+bool train_counts_tiles(int64_t total) { return total > 2 * kTrainSms; }
+
 template <int BN, bool kBias, bool kBF16, int kMask>
 int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                        BsaParams p, int n_tiles, cudaStream_t stream) {
@@ -1272,7 +1287,8 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   if (launch_regs * kThreads < 128 * static_cast<int>(kRegsCtl + kRegsSoftmax)) return SAF_ERR_UNSUPPORTED;
   const int sms = current_device_sms();
   if (sms <= 0) return SAF_ERR_CUDA;
-  if ((rc = tile_counter_slot(&p.tile_ctr)) != SAF_OK) return rc;
+  if constexpr (kMask != kMaskTrain)
+    if ((rc = tile_counter_slot(&p.tile_ctr)) != SAF_OK) return rc;
   p.n_tiles = n_tiles;
   p.BH = p.B * p.H;
   // Lead tiles (dense text rows: every key block) are the longest work items;
@@ -1285,13 +1301,8 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   if (lead > 0 && kMask != kMaskPool && kMask != kMaskKeys) {
     const int64_t items = static_cast<int64_t>(lead) * p.BH;
     const int sp = kMask == kMaskTrain ? train_split_cap(items, p.Sk) : split_cap(items, sms);
-    // the training forward brings its own buffers, so that its launches may
-    // overlap (the host entry sized them by the same rule)
     if (kMask == kMaskTrain) {
-      if (sp > 1 && p.split_part != nullptr) {
-        SAF_CUDA_TRY(cudaMemsetAsync(p.split_cnt, 0, static_cast<size_t>(items * kBM) * sizeof(int), stream));
-        p.splits = sp;
-      }
+      if (sp > 1 && p.split_part != nullptr) p.splits = sp;
     } else if (sp > 1 && items * sp * kBM * kSplitRow <= kSplitFloats && items * kBM <= kSplitCnts) {
       if ((rc = split_buffers(&p.split_part, &p.split_cnt)) != SAF_OK) return rc;
       SAF_CUDA_TRY(cudaMemsetAsync(p.split_cnt, 0, static_cast<size_t>(items * kBM) * sizeof(int), stream));
@@ -1299,7 +1310,16 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
     }
   }
   const int64_t total = (static_cast<int64_t>(lead) * p.splits + n_tiles - lead) * p.BH;
-  const int grid = static_cast<int>(total < 2 * sms ? total : 2 * sms);  // two CTAs per SM
+  int grid = static_cast<int>(total < 2 * sms ? total : 2 * sms);  // two CTAs per SM
+  if constexpr (kMask == kMaskTrain) {
+    // the training forward brings its own buffers, so that its launches may
+    // overlap, replays of captured ones included (sized by bsa_train_space)
+    if (p.tile_ctr == nullptr) grid = static_cast<int>(total);
+    const size_t cnt = p.splits > 1 ? static_cast<size_t>(lead) * p.BH * kBM * sizeof(int) : 0;
+    const size_t clear = cnt + (p.tile_ctr != nullptr ? sizeof(unsigned int) : 0);  // they lie side by side
+    void* at = cnt > 0 ? static_cast<void*>(p.split_cnt) : static_cast<void*>(p.tile_ctr);
+    if (clear > 0) SAF_CUDA_TRY(cudaMemsetAsync(at, 0, clear, stream));
+  }
   kern<<<grid, kThreads, smem, stream>>>(mq, mk, mv, p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
@@ -1307,13 +1327,19 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
 
 }  // namespace
 
-// Bytes of the split buffers of a training forward (0: its lead tiles run
-// unsplit): partial rows, then one counter per lead row.
-int64_t bsa_train_split_bytes(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles, int64_t* part_bytes) {
-  const int64_t items = std::min<int64_t>(lead_tiles, (Sq + kBM - 1) / kBM) * BH;
+// A training forward's buffers: partial rows and one counter per lead row
+// where its lead tiles may be split, and the next-tile counter (16 bytes).
+TrainSpace bsa_train_space(int64_t BH, int64_t Sq, int64_t Sk, int64_t lead_tiles) {
+  const int64_t tiles = (Sq + kBM - 1) / kBM;
+  const int64_t items = std::min<int64_t>(lead_tiles, tiles) * BH;
   const int sp = items > 0 ? train_split_cap(items, Sk) : 1;
-  *part_bytes = sp > 1 ? items * sp * kBM * kSplitRow * static_cast<int64_t>(sizeof(float)) : 0;
-  return sp > 1 ? *part_bytes + items * kBM * static_cast<int64_t>(sizeof(int)) : 0;
+  TrainSpace s{};
+  if (sp > 1) {
+    s.part = items * sp * kBM * kSplitRow * static_cast<int64_t>(sizeof(float));
+    s.cnt = items * kBM * static_cast<int64_t>(sizeof(int));
+  }
+  if (train_counts_tiles(items * (sp - 1) + tiles * BH)) s.tile = 16;
+  return s;
 }
 
 // Host entry for 16-bit inputs (validated by the caller in saf_api.cu).
@@ -1382,6 +1408,7 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
     p.lse = train->lse;
     p.split_part = train->split_part;
     p.split_cnt = train->split_cnt;
+    p.tile_ctr = train->tile_ctr;
   }
   if (pool != nullptr && (bias || frames != nullptr || row_ranges != nullptr)) return SAF_ERR_UNSUPPORTED;
 #define SAF_BSA_CASE(BN_, BIAS_, BF_, MASK_)                               \

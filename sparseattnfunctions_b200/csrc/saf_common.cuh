@@ -93,12 +93,21 @@ struct PoolArgs {
 };
 
 // Training forward of the attention kernels: the row log-sum-exp output
-// [B*H, Sq] and the caller's buffers for split tiles: partial rows and counters
-// (null when every tile runs unsplit).
+// [B*H, Sq] and the caller's buffers: partial rows and counters of split tiles
+// (null when every tile runs unsplit), and the 16-bit kernel's next-tile
+// counter (null when every CTA has one work item).
 struct TrainArgs {
   float* lse;
   float* split_part;
   int* split_cnt;
+  unsigned int* tile_ctr;
+};
+
+// The training forward's workspace: partial rows, counters of split tiles,
+// next-tile counter (bytes; all are 0 where nothing is needed).
+struct TrainSpace {
+  int64_t part, cnt, tile;
+  int64_t bytes() const { return part + cnt + tile; }
 };
 
 // Common checks of a [B,H,S,D] view: non-null, D-stride 1 implied, positive

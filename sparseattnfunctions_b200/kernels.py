@@ -466,12 +466,11 @@ def bsa_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, csr: BlockCSR
         return out.zero_(), lse.fill_(-math.inf)
     lib = _lib.load()
     tq, tk, tv, to = _p4(q, B, H, Sq, D), _p4(k, B, H, Sk, D), _p4(v, B, H, Sk, D), _p4(out, B, H, Sq, D)
-    lead, ws_bytes, ws_ptr = int(csr.dense_rows), 0, None
-    if lead > 0 or q.dtype == torch.float32:
-        ws_bytes = lib.saf_bsa_fwd_lse_workspace_bytes(tq, tk, csr.block_m, lead)
-        if ws_bytes:
-            ws = q.new_empty(ws_bytes, dtype=torch.uint8)
-            ws_ptr = ws.data_ptr()
+    lead, ws_ptr = int(csr.dense_rows), None
+    ws_bytes = lib.saf_bsa_fwd_lse_workspace_bytes(tq, tk, csr.block_m, lead)
+    if ws_bytes:
+        ws = q.new_empty(ws_bytes, dtype=torch.uint8)
+        ws_ptr = ws.data_ptr()
     rc = lib.saf_bsa_fwd_lse(tq, tk, tv, to, csr.row_ptr.data_ptr(), csr.col_idx.data_ptr(), csr.col_idx.numel(),
                              csr.block_m, csr.block_n, sm_scale, lead, lse.data_ptr(), ws_ptr, ws_bytes,
                              _stream_ptr(dev))

@@ -88,3 +88,32 @@ def test_gradient_expanded_over_heads_or_batch(cuda_device, dtype):
     training.sparse_attention(*x, csr, 0.125).sum(1).mul(d[:, 0]).sum().backward()
     ref = kernels.bsa_bwd(d[:, :1].expand(d.shape).contiguous(), q, k, v, out, lse, csr, 0.125)
     assert all(torch.equal(a.grad, b) for a, b in zip(x, ref))
+
+
+@pytest.mark.parametrize("lead", [0, 2])
+def test_replays_beside_other_forwards(cuda_device, lead):
+    """Replays of a captured training forward on one stream beside more than 64
+    direct ones on another, more query tiles each than the GPU takes at once:
+    no launch shares a counter with another, so all give the bits of one alone."""
+    H, S = 20, 4000
+    q, k, v = (_randn(230 + i, 1, H, S, 64, dtype=BF16).to(cuda_device) for i in range(3))
+    mask = _mask(233, 1, H, 32, 32, 0.3)
+    mask[:, :, :lead] = True
+    csr = kernels.mask_to_csr(mask.to(cuda_device), 128, 128, dense_rows=lead)
+    ref = kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+    side = torch.cuda.Stream(cuda_device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        held = [kernels.bsa_fwd_lse(q, k, v, csr, 0.125) for _ in range(8)]
+    direct = []
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            graph.replay()
+        direct += [kernels.bsa_fwd_lse(q, k, v, csr, 0.125) for _ in range(8)]
+    torch.cuda.synchronize()
+    for out, lse in held + direct:
+        assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
