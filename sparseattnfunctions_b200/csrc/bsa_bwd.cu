@@ -74,7 +74,10 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
       w.part = reinterpret_cast<float*>(take(static_cast<size_t>(w.part_cap) * 2 * 128 * 64 * 4));
       w.split = reinterpret_cast<uint2*>(take(static_cast<size_t>(w.part_cap / 2) * 8));
     }
-    w.amax = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (w.Sp / 128)) * 4));
+    if (q->dtype == SAF_F16) {
+      w.stat_exp = reinterpret_cast<float*>(take(static_cast<size_t>(BH * w.Sp) * 4));
+      w.amax = reinterpret_cast<float*>(take(static_cast<size_t>(BH * (w.Sp / 64)) * 4));
+    }
   }
   if (q->dtype == SAF_F32) {
     const int64_t tk = (k->S + kT - 1) / kT, tq = (q->S + kT - 1) / kT;
@@ -245,7 +248,8 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, const __half*) {
 
 // -delta and the negative log-sum-exp of 128 rows of head g.  A row that sees
 // no key (lse -inf) and the rows that pad the last tile get -inf, so that
-// every exp(s - lse) of theirs is 0.  f16: also the rows' largest |do|.
+// every exp(s - lse) of theirs is 0.  f16: also what the rows' and the two
+// 64-row blocks' largest |do| ask for.
 template <typename T>
 __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -260,7 +264,8 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   };
   if constexpr (sizeof(T) == 2) {  // D = 64: 8 lanes of 16 bytes a row
     const int sub = lane & 7;
-    float amax = 0.f;
+    constexpr bool kMax = std::is_same<T, __half>::value;
+    float amax[2] = {0.f, 0.f};  // of the chunk's two 64-row blocks
     constexpr int kRows = kRowChunk / 32;  // a thread's rows, all in flight
     uint4 x[kRows], y[kRows];
 #pragma unroll
@@ -273,29 +278,39 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
-      float sum = 0.f;
+      float sum = 0.f, row_max = 0.f;
       const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 fx = unpack2(xs[e], static_cast<const T*>(nullptr));
         const float2 fy = unpack2(ys[e], static_cast<const T*>(nullptr));
         sum = fmaf(fx.x, fy.x, fmaf(fx.y, fy.y, sum));
-        amax = fmaxf(amax, fmaxf(fabsf(fy.x), fabsf(fy.y)));
+        if constexpr (kMax) row_max = fmaxf(row_max, fmaxf(fabsf(fy.x), fabsf(fy.y)));
       }
 #pragma unroll
       for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       if (sub == 0) store(row, sum);
+      if constexpr (kMax) {
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) row_max = fmaxf(row_max, __shfl_xor_sync(0xffffffffu, row_max, off));
+        if (sub == 0) p.w.stat_exp[base + row] = static_cast<float>(f16_ds_exponent(row_max));
+        amax[i / 2] = fmaxf(amax[i / 2], row_max);
+      }
     }
-    if constexpr (std::is_same<T, __half>::value) {
-      __shared__ float warp_max[8];
+    if constexpr (kMax) {
+      __shared__ float warp_max[2][8];
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-      if (lane == 0) warp_max[warp] = amax;
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int off = 16; off > 4; off >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], off));
+        if (lane == 0) warp_max[i][warp] = amax[i];
+      }
       __syncthreads();
-      if (threadIdx.x == 0) {
+      if (threadIdx.x < 2) {
+        float m = 0.f;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) amax = fmaxf(amax, warp_max[i]);
-        p.w.amax[g * (p.w.Sp / kRowChunk) + chunk] = amax;
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, warp_max[threadIdx.x][i]);
+        p.w.amax[g * (p.w.Sp / 64) + 2 * chunk + threadIdx.x] = m;
       }
     }
   } else {

@@ -29,7 +29,7 @@ struct BwdWorkspace {
   int32_t* count_q;
   int32_t* count_k;
   // 16-bit kernel only: work items by length (longest class first) and the
-  // counters, zeroed before the preparation; the largest |do| of each 128 rows
+  // counters, zeroed before the preparation
   uint2* items;          // [kClasses][item_cap]: (1 << 31 for dk / dv) | head * lines + line, part (see PartOf)
   int32_t* class_count;  // [kClasses]
   int32_t* next;         // the next item to take
@@ -40,7 +40,10 @@ struct BwdWorkspace {
   int32_t* parts_used;
   int32_t* split_count;  // lines cut
   uint2* split;          // [part_cap / 2]: the line as in items, its first part and their number
-  float* amax;           // [BH, Sp / 128]
+  // f16 only: the exponent that takes a row's largest |do| to [2^-4, 2^-3),
+  // and the largest |do| of each 64 rows
+  float* stat_exp;  // [BH, Sp]
+  float* amax;      // [BH, Sp / 64]
   float* part;  // partial sums
   // fp32 kernel only: CTAs that share a tile, and the tiles' counts of finished ones
   int chunks;
@@ -49,6 +52,10 @@ struct BwdWorkspace {
   int64_t Sp;  // Sq rounded up to 128
   size_t bytes;
 };
+
+// Exponent of the power of two that takes a largest |do| of a to [2^-4, 2^-3);
+// 0 where all are zero or not finite.
+__device__ __forceinline__ int f16_ds_exponent(float a) { return a > 0.f && a <= 65504.f ? -4 - ilogbf(a) : 0; }
 
 // Length classes of the work items: class 15 - floor(log2(blocks)), so that
 // the longest lists start first and the short ones fill the last wave.

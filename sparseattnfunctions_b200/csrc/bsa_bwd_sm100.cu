@@ -33,7 +33,13 @@
 //
 // f16: p below 2^-14 and ds of small gradients would leave the type's normal
 // range, so P is formed times 2^4 and dS times a power of two that takes the
-// head's largest |do| to [2^-4, 2^-3); the outputs are scaled back.
+// largest |do| to [2^-4, 2^-3); the outputs are scaled back.  In dq items that
+// is the row's own largest (a row is one thread's, and its power goes into the
+// exponent of P), in dk items the largest of the blocks listed for the key's
+// half of the tile, so that a few rows with a large gradient take no bits from
+// the others (with one power for the whole head, rows 2^12 below its largest
+// were left with four bits).  dS then stays
+// below 256 times the largest |v|.
 //
 // P and dS are rounded to the 16-bit type because the tensor cores want A and B
 // of one type (walk1 and walk2 are the caller's); the sums over them, S, dP,
@@ -92,9 +98,9 @@ struct Item {
   int32_t keys;  // 1: dk and dv of a key tile, 0: dq of a query tile, -1: no more items
   int32_t g, tile;
   int32_t n;     // walked tiles
-  float ds_scale;
   int32_t part;  // -1, or where the fp32 sums of this part of a line go
-  int32_t pad[2];
+  int32_t ds_exp[2];  // f16, dk: exponent of dS's power of two for each half of the own tile
+  int32_t pad;
 };
 
 struct BwdParams {
@@ -361,8 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int n_items = mine;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) n_items += __shfl_xor_sync(0xffffffffu, n_items, o);
-      int it = 0, t = 0, nown = 0, amax_g = -1;
-      float ds_scale = 1.f;
+      int it = 0, t = 0, nown = 0;
       bool ok = true;
       int lin = lane == 0 ? atomicAdd(p.w.next, 1) : 0;
       while (ok) {
@@ -401,17 +406,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             n = min(n - t0 * per, (t1 - t0) * per);
             im.n = t1 - t0;
           }
-          if (!kBF16 && im.g != amax_g) {
-            amax_g = im.g;
-            const int chunks = static_cast<int>(p.w.Sp / 128);
-            float a = 0.f;
-            for (int i = lane; i < chunks; i += 32) a = fmaxf(a, p.w.amax[static_cast<int64_t>(im.g) * chunks + i]);
+          if (!kBF16 && im.keys) {  // the largest |do| of the listed query blocks
+            const float* amax = p.w.amax + im.g * (p.w.Sp / kUnit);
+            const int per = block / kUnit;
+            float a0 = 0.f, a1 = 0.f;
+#pragma unroll 4
+            for (int i = lane; i < n; i += 32) {
+              const uint32_t ent = list[i];
+              const float* at = amax + (ent & 0x3fffu) * per;
+              const float x = fmaxf(at[0], at[per - 1]);
+              if (ent & 0x4000u) a0 = fmaxf(a0, x);
+              if (ent & 0x8000u) a1 = fmaxf(a1, x);
+            }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            // exponent of the largest |do| -> [2^-4, 2^-3); all zero or not finite: unscaled
-            ds_scale = a > 0.f && a <= 65504.f ? ldexpf(1.f, -4 - ilogbf(a)) : 1.f;
+            for (int o = 16; o > 0; o >>= 1) {
+              a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, o));
+              a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, o));
+            }
+            im.ds_exp[0] = f16_ds_exponent(a0);
+            im.ds_exp[1] = f16_ds_exponent(a1);
           }
-          im.ds_scale = ds_scale;
         }
         if (lane == 0 && lin < n_items) lin = atomicAdd(p.w.next, 1);  // the next one, in flight over this one
         const int slot = it & 1;
@@ -626,13 +640,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!c.wait_all(c.own_full(slot), (it >> 1) & 1)) break;
       const int keys = c.items[slot].keys, n = c.items[slot].n;
       if (keys < 0) break;
-      const float ds_scale = kBF16 ? 1.f : c.items[slot].ds_scale;
+      // f16: dS's power of two, for this half of the own tile (dk) or this thread's row (dq)
+      float ds_exp = kBF16 ? 0.f : static_cast<float>(c.items[slot].ds_exp[quarter >> 1]);
       if (keys) {
+        const float ds_scale = kBF16 ? 1.f : exp2f(ds_exp);
         for (int j = 0; j < n; ++j, ++t) compute_tile<true, kBF16>(c, p, w, quarter, t, 0.f, 0.f, ds_scale);
       } else {
         const int64_t at = c.items[slot].g * p.w.Sp + c.items[slot].tile * kM + row;
         // dS's power of two goes into the exponent: dq does not need P itself
-        const float nl = p.w.stat_lse[at] + (kBF16 ? 0.f : static_cast<float>(ilogbf(ds_scale)));
+        if constexpr (!kBF16) ds_exp = p.w.stat_exp[at];
+        const float nl = p.w.stat_lse[at] + ds_exp;
         const float nd = p.w.stat_delta[at];
         for (int j = 0; j < n; ++j, ++t) compute_tile<false, kBF16>(c, p, w, quarter, t, nl, nd, 1.f);
       }
@@ -655,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; ++e) r[e] = 0u;
       }
       const float unscale = kBF16 ? 1.f : 1.f / kF16PScale;
-      const float scale = dv ? unscale : kBF16 ? p.scale : p.scale * unscale / ds_scale;
+      const float scale = dv ? unscale : kBF16 ? p.scale : p.scale * unscale * exp2f(-ds_exp);
       const int part = kParts ? c.items[slot].part : -1;
       if (kParts && part >= 0) {  // sums of a part of the line: fp32, scaled, to the workspace
         if (keys || (w & 1) == 0) {  // dq: one of the two warpgroups that hold the same 32 channels

@@ -5,6 +5,7 @@ Tolerances as in test_gpu_training.py unless a test derives its own.
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -117,3 +118,40 @@ def test_replays_beside_other_forwards(cuda_device, lead):
     torch.cuda.synchronize()
     for out, lse in held + direct:
         assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+
+
+def _row_errors(got, ref):
+    """Largest error of a row over the row's own size (2-norms)."""
+    got = got.double().cpu().numpy()
+    size = np.linalg.norm(ref, axis=-1)
+    return float((np.linalg.norm(got - ref, axis=-1)[size > 0] / size[size > 0]).max())
+
+
+@pytest.mark.parametrize("bm,bn", [(128, 128), (64, 64), (64, 128), (128, 64)])
+@pytest.mark.parametrize("large", [2.0 ** 4, 2.0 ** 8, 2.0 ** 12])
+@pytest.mark.parametrize("H,S", [(4, 1500), (1, 4000)])
+def test_f16_rows_of_unlike_size(cuda_device, bm, bn, large, H, S):
+    """One row block's gradients ``large`` times the others': every row of dq is
+    good to its own size, and so are dk and dv of every key.
+
+    A row's error is made of the rounding of the result and those of its terms
+    ds or p, each at most u / sqrt(3) of the power of two above it in the mean
+    square: 0.816 u together for values without a common part.  The rms of 64
+    channels spreads by 1 / sqrt(128), 1.4 at 4.5 of it; what falls below f16's
+    normal range is 2^-25 beside terms of 2^-9 and the fp32 sums 4e-5 of them,
+    0.05 u."""
+    q, k, v, dout = (_randn(240 + i, 1, H, S, 64, dtype=torch.float32) for i in range(4))
+    dout[:, :, 2 * bm:3 * bm] *= large
+    q, k, v, dout = (t.to(F16) for t in (q, k, v, dout))
+    nbq, nbk = math.ceil(S / bm), math.ceil(S / bn)
+    mask = _mask(244, 1, H, nbq, nbk, 0.3)
+    mask[..., 1] = True
+    mask[:, :, 2, nbk // 2:] = False
+    csr = kernels.mask_to_csr(mask.to(cuda_device), bm, bn)
+    gq, gk, gv, gd = (t.to(cuda_device) for t in (q, k, v, dout))
+    out, lse = kernels.bsa_fwd_lse(gq, gk, gv, csr, 0.125)
+    grads = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)
+    live = otr.token_mask(mask, S, S, bm, bn)
+    ref = otr.attention_grad(dout, q, k, v, out.cpu(), lse.cpu(), live, 0.125)
+    off = {n: _row_errors(x, ref[n][0]) / U[F16] for n, x in zip(("dq", "dk", "dv"), grads)}
+    assert max(off.values()) <= 1.2, off
