@@ -46,11 +46,12 @@
 // lse and delta are fp32.  Against sums of unrounded values that makes the
 // error of dk and dv 1.4 times the output's own rounding.  A row of dS sums to
 // zero, so in dq a component that all keys share cancels, but its share of the
-// rounding does not (keys that vary smoothly: 1.5 times the output's rounding,
-// more with a larger common part).  In bf16, dq therefore adds the product of
-// what the rounding took off too, from P's columns, which its items leave free:
-// 1.0 times, and 2.83 instead of 2.61 ms at the size below.  f16 rounds eight
-// times finer and goes without (4 heads of 33976 tokens, strided: 0.61 ms).
+// rounding does not: with keys whose common part is eight times their spread, dq
+// was off by 3.3 (bf16) and 3.4 to 3.7 (f16) times the output's rounding.  dq
+// therefore adds the product of what the rounding took off too, from P's
+// columns, which its items leave free: 1.0 times.  That costs 2.83 instead of
+// 2.61 ms at the bf16 size below, and 735 instead of 661 us a call at 4 heads of
+// 33976 tokens in f16 (strided).
 //
 // Bound (2 x 30 heads of 17776 tokens, a tenth of the 128-blocks, bf16): the
 // tensor pipe, the exponentials and the issue slots share the SM, none of them
@@ -74,6 +75,8 @@
 //
 // Every wait is bounded, as in the forward kernel.
 #include "bsa_bwd.cuh"
+
+#include <cuda_fp16.h>
 
 namespace saf {
 namespace {
@@ -233,14 +236,21 @@ __device__ __forceinline__ void zero16(uint32_t (&r)[16]) {
   for (int e = 0; e < 16; ++e) asm volatile("mov.b32 %0, 0;" : "=r"(r[e]));
 }
 
+// What rounding to the 16-bit type took off a pair.
+template <bool kBF16>
+__device__ __forceinline__ f2 rounded_off(f2 x, uint32_t r) {
+  if constexpr (kBF16) return pair(first(x) - __uint_as_float(r << 16), second(x) - __uint_as_float(r & 0xffff0000u));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&r));
+  return pair(first(x) - y.x, second(x) - y.y);
+}
+
 // One tile: 32 columns of this thread's row; t is the tile's number in the
 // CTA.  kKeys: lse and delta per column (shared
 // memory; the MMA thread that arrives on `scores` has waited for the stage),
-// and P goes to TMEM too.  dq in bf16: the low part of dS takes P's place.
+// and P goes to TMEM too.  dq: the low part of dS takes P's place.
 template <bool kKeys, bool kBF16>
 __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, uint32_t t,
                                              float nl_row, float nd_row, float ds_scale) {
-  constexpr bool kLow = !kKeys && kBF16;
   const uint32_t s = t % kStages, par = t & 1;
   const uint32_t lane_addr = c.tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const uint32_t ts = lane_addr + w * kCols;
@@ -276,15 +286,12 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
       f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
       if constexpr (!kBF16 && kKeys) z = mul2(z, mk2(ds_scale, ds_scale));
       dk[e / 2] = pack2<kBF16>(z);
-      if constexpr (kLow) {  // what rounding takes off dS
-        pk[e / 2] = pack2<kBF16>(pair(first(z) - __uint_as_float(dk[e / 2] << 16),
-                                      second(z) - __uint_as_float(dk[e / 2] & 0xffff0000u)));
-      }
+      if constexpr (!kKeys) pk[e / 2] = pack2<kBF16>(rounded_off<kBF16>(z, dk[e / 2]));
     }
   }
   if (!((ent.y >> (quarter >> 1)) & 1)) {  // not listed for this half of the own tile, or no second unit
     zero16(dk);
-    if constexpr (kKeys || kLow) zero16(pk);
+    zero16(pk);
   }
   if constexpr (!kKeys) {
     // keys past the end: their scores are 0, not -inf
@@ -294,13 +301,13 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
       for (int e = 0; e < kCols / 2; ++e) {
         const uint32_t live = 2 * e + 1 < valid ? 0xffffffffu : 2 * e < valid ? 0xffffu : 0u;
         dk[e] &= live;
-        if constexpr (kLow) pk[e] &= live;
+        pk[e] &= live;
       }
     }
   }
   pass(c, c.added(), par ^ 1);  // the tile before is multiplied
   tc_fence_after();
-  if constexpr (kKeys || kLow) tmem_st16(tp + kColP, pk);
+  tmem_st16(tp + kColP, pk);
   tmem_st16(tp + kColDS, dk);
   tmem_wait_st();
   tc_fence_before();
@@ -583,8 +590,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
               add(kColK, kColDS, b, both, j > 0);
             } else {
-              if (kBF16) add(kColK, kColP, b, both, j > 0);  // what rounding took off dS
-              add(kColK, kColDS, b, both, kBF16 || j > 0);
+              add(kColK, kColP, b, both, j > 0);  // what rounding took off dS
+              add(kColK, kColDS, b, both, 1u);
             }
             tc_commit(c.added());
             tc_commit(c.empty(s));
