@@ -992,16 +992,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 #if SAF_OVERFLOW_GUARD
       // Speculative P with the running max, no block maximum: the max moves
       // only for a row whose block sum shows P could approach overflow
-      // (> 2^64; the normalised result does not depend on which max P was
-      // taken against).  The pooled map needs every block's maximum, so that
+      // (> 2^64, in f16 > 2^15; the normalised result does not depend on
+      // which max P was taken against).  The pooled map needs every block's maximum, so that
       // mode keeps the threshold rule below.
       constexpr bool kGuard = kMask != kMaskPool;
 #else
       constexpr bool kGuard = false;
 #endif
-      // The training mode keeps f16 P inside the type's range (65504): its
-      // rows move their max once a block sum passes 2^15.
-      constexpr float kGuardMax = kMask == kMaskTrain && !kBF16 ? 32768.f : 1.8446744e19f;
+      // P is stored in the input type: bf16 has fp32's exponents, f16 ends at 65504
+      constexpr float kGuardMax = kBF16 ? 1.8446744e19f : 32768.f;
       if (spec) {
         if (!exp_pass(-m_run, !kGuard, false)) {
           ok = false;
@@ -1012,7 +1011,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       bool upd;
       if (kGuard && spec) {
-        upd = !(lo2(rs) + hi2(rs) <= kGuardMax);  // 2^64; catches inf and NaN too
+        upd = !(lo2(rs) + hi2(rs) <= kGuardMax);  // catches inf and NaN too
         if (__any_sync(0xffffffffu, upd)) mx = block_max() * sl2;
       } else {
         mx *= sl2;

@@ -10,8 +10,11 @@ import pytest
 import torch
 
 from oracle import training as otr
+from oracle.selection import to_f64
 from sparseattnfunctions_b200 import kernels, training
-from test_gpu_training import BF16, F16, U, _check_fwd, _check_grad, _mask, _randn  # noqa: F401
+from sparseattnfunctions_b200.geometry import VideoGeometry
+from sparseattnfunctions_b200.special_attentions.block_mask_attn import BlockSparseAttention
+from test_gpu_training import BF16, F16, U, _check_grad, _mask, _near, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +179,50 @@ def test_f16_keys_with_a_common_part(cuda_device, H, Sq, Sk, bm, bn):
     ref = otr.attention_grad(dout, q, k, v, out.cpu(), lse.cpu(), live, 0.125)["dq"][0]
     off = np.linalg.norm(dq.double().cpu().numpy() - ref) / np.linalg.norm(ref)
     assert off <= 0.65 * U[F16], f"{off / U[F16]:.3f} U"
+
+
+@pytest.mark.parametrize("bn", [64, 128])
+@pytest.mark.parametrize("mode", ["plain", "lead", "bias", "ranges", "frames", "pool", "keys", "train", "processor"])
+def test_f16_scores_that_grow_along_the_keys(cuda_device, mode, bn):
+    """Later key blocks exceed a row's first ones by far more than f16's range
+    (2^16): finite, and right, in every form of the 16-bit forward."""
+    geo = VideoGeometry(64, 4, 10, 16)
+    H, S = 2, geo.seq_len
+    q, k, v = (_randn(260 + i, 1, H, S, 64, dtype=torch.float32) for i in range(3))
+    k[:, :, :bn] *= 0.05
+    k[:, :, bn:] *= 6.0
+    q, k, v = (t.to(F16) for t in (q, k, v))
+    gq, gk, gv = (t.to(cuda_device) for t in (q, k, v))
+    nb = math.ceil(S / bn)
+    csr = kernels.mask_to_csr(torch.ones(1, H, nb, nb, dtype=torch.bool, device=cuda_device), bn, bn,
+                              dense_rows=2 if mode == "lead" else 0)
+    live = np.ones((1, H, S, S), dtype=bool)
+    lse = None
+    if mode in ("plain", "lead"):
+        out = kernels.bsa_fwd(gq, gk, gv, csr, 0.125)
+    elif mode == "bias":
+        out = kernels.bsa_fwd(gq, gk, gv, csr, 0.125, kv_bias=torch.zeros(S, device=cuda_device))
+    elif mode == "ranges":
+        live[..., S - 30:] = False
+        ranges = torch.tensor([[0, S - 30, 0, 0]], dtype=torch.int32, device=cuda_device).repeat(S, 1)
+        out = kernels.bsa_fwd(gq, gk, gv, csr, 0.125, row_ranges=ranges)
+    elif mode == "frames":
+        bits = torch.full((H, geo.frames), 15, dtype=torch.int32, device=cuda_device)
+        fm = kernels.FrameMask(bits, None, None, geo.text_len, geo.frames, geo.frame_len)
+        out = kernels.bsa_fwd_frames(gq, gk, gv, kernels.frame_csr(fm, 1, H, bn, bn), fm, 0.125)
+    elif mode == "pool":
+        out = kernels.bsa_fwd_pool(gq, gk, gv, csr, 0.125)[0]
+    elif mode == "keys":
+        keys = torch.arange(S, dtype=torch.int32, device=cuda_device)[None]
+        out = kernels.bsa_fwd_keys(gq, gk, gv, keys, torch.zeros(1, dtype=torch.int32, device=cuda_device), 0.125)
+    elif mode == "train":
+        out, lse = kernels.bsa_fwd_lse(gq, gk, gv, csr, 0.125)
+    else:
+        out = BlockSparseAttention(block_size=bn, density=1.0, geometry=geo)(gq, gk, gv)
+    ref, ref_lse = otr.attention(q, k, v, live, 0.125)
+    # as test_gpu_training.py bounds the forward: the output's rounding, and P's
+    # with an exponential good to 1e-4, doubled for the second order
+    tol = U[F16] * np.abs(ref) + 2 * (U[F16] + 1e-4) * np.abs(to_f64(v)).max(axis=2, keepdims=True) + 1e-6
+    _near("out", out, ref, tol)
+    if lse is not None:
+        _near("lse", lse, ref_lse, 1e-4)
