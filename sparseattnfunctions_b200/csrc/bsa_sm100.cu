@@ -1008,6 +1008,16 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       } else {
         mx = block_max();
+        // a maximum passes over NaN: a row with nothing but NaN (and masked
+        // keys) would look like one that sees nothing
+        if constexpr (kMask == kMaskTrain) {
+          if (mx == -INFINITY) {
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < BN; ++e) sum += t[e];
+            if (sum != sum) l_run = sum;
+          }
+        }
       }
       bool upd;
       if (kGuard && spec) {
@@ -1122,7 +1132,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         float mm = -INFINITY;
         for (int sp = 0; sp < n_split; ++sp) {
           const float ls = __ldcg(base + sp * sstride + kD + 1);
-          if (ls > 0.f) mm = fmaxf(mm, __ldcg(base + sp * sstride + kD));
+          if (ls != 0.f) mm = fmaxf(mm, __ldcg(base + sp * sstride + kD));
         }
         float acc[kD];
 #pragma unroll
@@ -1131,7 +1141,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int sp = 0; sp < n_split; ++sp) {
           const float* ps = base + sp * sstride;
           const float ls = __ldcg(ps + kD + 1);
-          if (!(ls > 0.f)) continue;
+          if (ls == 0.f) continue;  // no visible key (NaN goes on into the row)
           const float wgt = ex2_approx(__ldcg(ps + kD) - mm);
           ll += ls * wgt;
 #pragma unroll

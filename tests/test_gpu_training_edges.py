@@ -14,7 +14,7 @@ from oracle.selection import to_f64
 from sparseattnfunctions_b200 import kernels, training
 from sparseattnfunctions_b200.geometry import VideoGeometry
 from sparseattnfunctions_b200.special_attentions.block_mask_attn import BlockSparseAttention
-from test_gpu_training import BF16, F16, U, _check_grad, _mask, _near, _randn
+from test_gpu_training import BF16, F16, F32, U, _check_grad, _mask, _near, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -226,3 +226,40 @@ def test_f16_scores_that_grow_along_the_keys(cuda_device, mode, bn):
     _near("out", out, ref, tol)
     if lse is not None:
         _near("lse", lse, ref_lse, 1e-4)
+
+
+@pytest.mark.parametrize("dtype,bm,S,lead", [(BF16, 128, 600, 0), (F16, 64, 600, 0), (BF16, 128, 3500, 2), (F16, 64, 3500, 3),
+                                             (F32, 64, 600, 0), (F32, 128, 3500, 0)])
+def test_nan_reaches_every_row_that_sees_it(cuda_device, dtype, bm, S, lead):
+    """A query row of NaN, and a NaN among the keys of a listed block: the rows
+    that see it have NaN output, log-sum-exp and dq, whether their keys are
+    walked in one piece or in several, and the other rows keep their bits."""
+    H = 2
+    q, k, v, dout = (_randn(270 + i, 1, H, S, 64, dtype=dtype).to(cuda_device) for i in range(4))
+    nb = math.ceil(S / bm)
+    mask = _mask(274, 1, H, nb, nb, 0.4)
+    mask[:, :, :lead] = True
+    mask[:, :, lead:, nb - 1] = False
+    mask[:, 1, lead:lead + 2, nb - 1] = True
+    csr = kernels.mask_to_csr(mask.to(cuda_device), bm, bm, dense_rows=lead)
+    clean, clean_lse = kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+    clean_dq = kernels.bsa_bwd(dout, q, k, v, clean, clean_lse, csr, 0.125)[0]
+
+    def check(q, k, seen):
+        out, lse = kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+        assert bool(torch.isnan(lse[seen]).all()) and bool(torch.isnan(out[seen]).all())
+        assert torch.equal(lse[~seen], clean_lse[~seen]) and torch.equal(out[~seen], clean[~seen])
+        dq = kernels.bsa_bwd(dout, q, k, v, out, lse, csr, 0.125)[0]
+        assert bool(torch.isnan(dq[seen]).all())
+        return dq
+
+    rows = torch.zeros(1, H, S, dtype=torch.bool, device=cuda_device)
+    rows[0, 0, 5] = rows[0, 1, S - 1] = True
+    bad = q.clone()
+    bad[rows] = float("nan")
+    dq = check(bad, k, rows)
+    assert torch.equal(dq[~rows], clean_dq[~rows])
+    seen = mask[..., nb - 1].to(cuda_device).repeat_interleave(bm, 2)[:, :, :S]
+    bad = k.clone()
+    bad[:, :, S - 1] = float("nan")
+    check(q, bad, seen)
