@@ -8,9 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-
 #include "../../include/saf_api.h"
+#include "smem_limit.cuh"
 
 #define SAF_CUDA_TRY(expr)                               \
   do {                                                   \
@@ -60,15 +59,13 @@ class DeviceScope {
 // microsecond a launch).
 template <auto kKernel>
 int32_t allow_smem(int bytes) {
-  static std::atomic<int> allowed[64] = {};
+  static SmemLimit limit;
   int dev = 0;
   SAF_CUDA_TRY(cudaGetDevice(&dev));
-  const bool known = dev >= 0 && dev < 64;
-  if (!known || allowed[dev].load(std::memory_order_relaxed) < bytes) {
-    SAF_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (known) allowed[dev].store(bytes, std::memory_order_relaxed);
-  }
-  return SAF_OK;
+  return limit.raise(dev, bytes, [](int n) -> int {
+    SAF_CUDA_TRY(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, n));
+    return SAF_OK;
+  });
 }
 
 inline int elem_bytes(int32_t dtype) { return dtype == SAF_F32 ? 4 : 2; }
