@@ -200,7 +200,8 @@ int32_t saf_bsa_fwd(const saf_tensor4* q, const saf_tensor4* k, const saf_tensor
 
 /* Training forward: saf_bsa_fwd without a bias that also stores the natural
  * log-sum-exp of every row, lse fp32 [B*H, Sq] contiguous, for saf_bsa_bwd.
- * Unlike saf_bsa_fwd, a row with no live key gives o = 0 and lse = -inf.
+ * Unlike saf_bsa_fwd, a row with no live key gives o = 0 and lse = -inf, and
+ * NaN or infinities reach the rows whose lists hold them, no others.
  * sm_scale is positive and finite.  workspace (16-byte aligned, of
  * saf_bsa_fwd_lse_workspace_bytes; 0 bytes: may be null) holds the partial
  * rows of split tiles and the launch's counters.  Nothing is shared between
@@ -223,7 +224,8 @@ int32_t saf_bsa_fwd_lse(const saf_tensor4* q, const saf_tensor4* k, const saf_te
  * q, k, v, out, lse as the forward had and left them (lse rows of head
  * b*H + h at lse_stride_bh >= Sq floats), dout the gradient of
  * out; dq, dk, dv are written whole (rows and keys that no block lists get
- * zeros).  p is recomputed; a listed column counts once however often its
+ * zeros; NaN and infinities stay with the rows and keys whose lists hold
+ * them).  p is recomputed; a listed column counts once however often its
  * row lists it.  No atomics touch the gradients: equal inputs give equal
  * bits.  bf16 / f16: D = 64, block sizes 64 or 128, 16-byte aligned rows.
  * f32: D = 64 or 128, block sizes multiples of 64.  At most 16384 blocks a

@@ -73,6 +73,13 @@
 // kind of item that adds its share of dq in memory would save two of the
 // products, but wants fp32 atomics, whose order changes the bits from run to run.
 //
+// Own tiles of two 64-token blocks: a half that does not list a walked unit has
+// zeros for it, formed without the exponentials (16 heads of 8000 tokens, 15 %
+// of the 64-blocks: 329 us, 363 with them).  0 times an infinity or NaN of the
+// unit would reach that half all the same, so tiles whose S or dP show one are
+// multiplied half by half, with the other half's lanes left out; done for every
+// tile, that cost 8 % at the size above.
+//
 // Every wait is bounded, as in the forward kernel.
 #include "bsa_bwd.cuh"
 
@@ -96,6 +103,7 @@ constexpr int kLaunchRegs = 96;
 static_assert(128 * kRegsCtl + 32 * kComputeWarps * kRegsCompute <= kThreads * kLaunchRegs, "register split");
 constexpr uint32_t kColS = 0, kColDP = 128, kColP = 256, kColDS = 320, kColV = 384, kColK = 448, kTmemCols = 512;
 constexpr float kF16PScale = 16.f;
+constexpr int kOdd = 4;  // in a unit's entry, beside the halves: its rows hold infinities or NaN
 
 struct Item {
   int32_t keys;  // 1: dk and dv of a key tile, 0: dq of a query tile, -1: no more items
@@ -155,7 +163,8 @@ __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_g
 struct Ctx {
   uint32_t bar0, own, walk, stat;
   Item* items;  // [2]
-  int2* ents;   // [kStages][2 units]: first walked row, live halves of the own tile (0: no second unit)
+  int2* ents;   // [kStages][2 units]: first walked row, halves of the own tile that list it (0: no second unit)
+  uint32_t* seen;  // [2 slots]: halves of the item's own tile whose sums were started
   const float* stats;
   volatile int* abort_flag;
   uint32_t tmem;
@@ -247,7 +256,10 @@ __device__ __forceinline__ f2 rounded_off(f2 x, uint32_t r) {
 // One tile: 32 columns of this thread's row; t is the tile's number in the
 // CTA.  kKeys: lse and delta per column (shared
 // memory; the MMA thread that arrives on `scores` has waited for the stage),
-// and P goes to TMEM too.  dq: the low part of dS takes P's place.
+// and P goes to TMEM too.  dq: the low part of dS takes P's place.  A half
+// of the own tile that does not list a unit has zeros there; infinities or NaN
+// in the unit's rows (every row of S or dP shows them) are noted in its entry,
+// since 0 times them would be NaN.
 template <bool kKeys, bool kBF16>
 __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, int w, int quarter, uint32_t t,
                                              float nl_row, float nd_row, float ds_scale) {
@@ -269,29 +281,35 @@ __device__ __forceinline__ void compute_tile(const Ctx& c, const BwdParams& p, i
   mbar_arrive(c.read());
   const f2 sl = mk2(p.scale_log2, p.scale_log2);
   uint32_t pk[kCols / 2], dk[kCols / 2];
-#pragma unroll
-  for (int e4 = 0; e4 < kCols / 4; ++e4) {
-    f2 ol[2] = {mk2(nl_row, nl_row), mk2(nl_row, nl_row)}, od[2] = {mk2(nd_row, nd_row), mk2(nd_row, nd_row)};
-    if constexpr (kKeys) {
-      const float4 l = nl[e4], d = nd[e4];
-      ol[0] = pair(l.x, l.y), ol[1] = pair(l.z, l.w);
-      od[0] = pair(d.x, d.y), od[1] = pair(d.z, d.w);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = 4 * e4 + 2 * i;
-      const f2 y = fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, ol[i]);
-      const f2 pr = pair(ex2_approx(first(y)), ex2_approx(second(y)));
-      if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(pr);
-      f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
-      if constexpr (!kBF16 && kKeys) z = mul2(z, mk2(ds_scale, ds_scale));
-      dk[e / 2] = pack2<kBF16>(z);
-      if constexpr (!kKeys) pk[e / 2] = pack2<kBF16>(rounded_off<kBF16>(z, dk[e / 2]));
-    }
-  }
   if (!((ent.y >> (quarter >> 1)) & 1)) {  // not listed for this half of the own tile, or no second unit
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e)
+      odd |= !(fabsf(__uint_as_float(r[e])) < INFINITY) || !(fabsf(__uint_as_float(rd[e])) < INFINITY);
+    if (odd && ent.y != 0) c.ents[2 * s + (w >> 1)].y = ent.y | kOdd;
     zero16(dk);
     zero16(pk);
+  } else {
+#pragma unroll
+    for (int e4 = 0; e4 < kCols / 4; ++e4) {
+      f2 ol[2] = {mk2(nl_row, nl_row), mk2(nl_row, nl_row)}, od[2] = {mk2(nd_row, nd_row), mk2(nd_row, nd_row)};
+      if constexpr (kKeys) {
+        const float4 l = nl[e4], d = nd[e4];
+        ol[0] = pair(l.x, l.y), ol[1] = pair(l.z, l.w);
+        od[0] = pair(d.x, d.y), od[1] = pair(d.z, d.w);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int e = 4 * e4 + 2 * i;
+        const f2 y = fma2(pair(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sl, ol[i]);
+        const f2 pr = pair(ex2_approx(first(y)), ex2_approx(second(y)));
+        if constexpr (kKeys) pk[e / 2] = pack2<kBF16>(pr);
+        f2 z = mul2(add2(pair(__uint_as_float(rd[e]), __uint_as_float(rd[e + 1])), od[i]), pr);
+        if constexpr (!kBF16 && kKeys) z = mul2(z, mk2(ds_scale, ds_scale));
+        dk[e / 2] = pack2<kBF16>(z);
+        if constexpr (!kKeys) pk[e / 2] = pack2<kBF16>(rounded_off<kBF16>(z, dk[e / 2]));
+      }
+    }
   }
   if constexpr (!kKeys) {
     // keys past the end: their scores are 0, not -inf
@@ -325,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
-  Ctx c{0, 0, 0, 0, nullptr, nullptr, nullptr, nullptr, 0, p};
+  Ctx c{0, 0, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, 0, p};
   c.bar0 = smem_u32(smem + L::kOffBar);
   c.own = smem_u32(smem);
   c.walk = smem_u32(smem + L::kOffWalk);
@@ -334,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   c.items = reinterpret_cast<Item*>(smem + L::kOffItem);
   c.ents = reinterpret_cast<int2*>(smem + L::kOffEnt);
   c.abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+  c.seen = reinterpret_cast<uint32_t*>(smem + L::kOffMisc + 8);
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(c.own_full(s), 1);
@@ -349,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(c.read(), 32 * kComputeWarps);
     mbar_init(c.written(), 32 * kComputeWarps);
     mbar_init(c.added(), 1);
-    mbar_init(c.acc_full(), 1);
+    mbar_init(c.acc_full(), 2);
     mbar_init(c.acc_empty(), kComputeWarps);
     *c.abort_flag = 0;
     fence_mbar_init();
@@ -554,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kIdesc = idesc_f16(kM, kD, kBF16, false, true);
         const uint32_t walk_lo = desc_lo(c.walk);
         // P or dS (TMEM column a) x walked tile (MN-major, b) added to column
-        // d; 16 walked rows a step, of one or both units
+        // d: 16 walked rows a step, of one or both units
         auto add = [&](uint32_t d, uint32_t a, uint32_t b, bool both, uint32_t accumulate) {
 #pragma unroll
           for (int kk = 0; kk < kUnit / 16; ++kk)
@@ -564,6 +583,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int kk = kUnit / 16; kk < kM / 16; ++kk)
               tc_mma_ts(c.tmem + d, c.tmem + a + kk * 8, desc64(b + kk * 128), kIdesc, 1u);
           }
+        };
+        // the same, each unit for the halves that list it alone
+        auto add_halves = [&](uint32_t d, uint32_t a, uint32_t b, uint32_t live0, uint32_t live1, uint32_t seen) {
+          constexpr int kSlices = kUnit / 16;
+          auto desc0 = [&](int kk) { return desc64(b + kk * 128); };
+          auto desc1 = [&](int kk) { return desc64(b + (kSlices + kk) * 128); };
+          tc_add_halves<kSlices>(c.tmem + d, c.tmem + a, desc0, kIdesc, live0, seen);
+          if (live1 != 0u)
+            tc_add_halves<kSlices>(c.tmem + d, c.tmem + a + kSlices * 8, desc1, kIdesc, live1, seen | live0);
         };
         uint32_t it = 0, t = 0, na = 0;  // na: items with tiles
         bool ok = true;
@@ -579,24 +607,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             ++na;
           }
+          uint32_t seen = 0u;  // halves of the own tile whose sums are started
           for (int j = 0; j < n; ++j, ++t) {
             const uint32_t s = t % kStages;
             const uint32_t b = walk_lo + s * (2 * L::kTile >> 4);
             ok = c.wait(c.written(), t & 1);
             if (!ok) break;
             tc_fence_after();
-            const bool both = c.ents[2 * s + 1].y != 0;
-            if (keys) {
-              add(kColV, kColP, b + (L::kTile >> 4), both, j > 0);
-              add(kColK, kColDS, b, both, j > 0);
-            } else {
-              add(kColK, kColP, b, both, j > 0);  // what rounding took off dS
-              add(kColK, kColDS, b, both, 1u);
+            const uint32_t e0 = c.ents[2 * s].y, e1 = c.ents[2 * s + 1].y;
+            const uint32_t b2 = keys ? b + (L::kTile >> 4) : b;
+            const uint32_t d2 = keys ? kColV : kColK;  // dq: P's columns hold what rounding took off dS
+            if (!((e0 | e1) & kOdd) && (seen == 3u || j == 0)) {
+              add(d2, kColP, b2, e1 != 0u, j > 0);
+              add(kColK, kColDS, b, e1 != 0u, !keys || j > 0);
+              seen = 3u;
+            } else {  // infinities or NaN that one half does not list
+              const uint32_t live0 = e0 & 3u, live1 = e1 & 3u, now = seen | live0 | live1;
+              add_halves(d2, kColP, b2, live0, live1, seen);
+              add_halves(kColK, kColDS, b, live0, live1, keys ? seen : now);
+              seen = now;
             }
             tc_commit(c.added());
             tc_commit(c.empty(s));
           }
-          if (ok && n > 0) tc_commit(c.acc_full());
+          if (ok && n > 0) {
+            c.seen[slot] = seen;
+            tc_commit(c.acc_full());
+            mbar_arrive(c.acc_full());  // hands on `seen`
+          }
         }
         tc_commit(c.drain(1));
         mbar_drain(c.drain(1), 0, p.status);
@@ -674,6 +712,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld(r);
         tc_fence_before();
         warp_arrive(c.acc_empty(), lane);
+        if (!((c.seen[slot] >> (quarter >> 1)) & 1u)) {  // nothing was ever added for this half
+#pragma unroll
+          for (int e = 0; e < 32; ++e) asm volatile("mov.b32 %0, 0;" : "=r"(r[e]));
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 32; ++e) r[e] = 0u;

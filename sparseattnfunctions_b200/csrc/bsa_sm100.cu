@@ -308,7 +308,12 @@ constexpr int kMaskPool = 4;
 // 0.88 ms at 2 x 30 heads of 17776 tokens, a tenth of the 128-blocks (0.620
 // TFLOP, 0.43 of the bf16 peak): bound as the mode without a mask, by the
 // exponentials and the hand-overs around them.
-constexpr int kMaskTrain = 5;
+// 128-row and 64-row mask blocks apart: the latter's tiles cover two mask rows,
+// and where one of them alone lists a key block, PV is added to its half alone
+// (0 times a NaN of V would reach the other).  16 heads of 8000 tokens, 15 % of
+// the 64-blocks: 196 us, 186 with PV added to both halves.
+constexpr int kMaskTrain = 5, kMaskTrain64 = 6;
+__host__ __device__ constexpr bool is_train(int mask) { return mask == kMaskTrain || mask == kMaskTrain64; }
 
 // TMA gather4: four rows (coordinates r0..r3 of a 2-D map whose box is one
 // row of 64 elements) into 4 x 128 bytes of shared memory, 128-byte swizzle
@@ -477,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     while (ok) {
       // next tile: fetched by lane 0, published in ring slot ti & 1
       int lin = 0;
-      if constexpr (kMask == kMaskTrain) {  // the first item without the counter
+      if constexpr (is_train(kMask)) {  // the first item without the counter
         if (ti == 0)
           lin = blockIdx.x;
         else if (p.tile_ctr == nullptr)
@@ -637,19 +642,24 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t tS = tmem + kColS, tO = tmem + kColO, tP = tmem + kColP;
 
       // O += P V for global block jg; `first` starts the tile's accumulator.
-      auto issue_pv = [&](int jg, bool first) -> bool {
+      // 64-row training mode: of the row halves `live` that list the block
+      // alone, started where not yet `seen`.
+      auto issue_pv = [&](int jg, bool first, uint32_t live, uint32_t seen) -> bool {
         const int sv = jg % kVS;
         const uint32_t pv = (jg / kVS) & 1;
         if (!mbar_wait(bar_v_full(sv), pv, abort_flag, p.status, p.budget_ns)) return false;
         if (!mbar_wait(bar_p_full, jg & 1, abort_flag, p.status, p.budget_ns)) return false;
         tc_fence_after();
         const uint32_t vbase = sV0 + sv * L::kKVBytes;
+        // B = V^T: N = D (contiguous, one 128B swizzle atom), K = kv rows;
+        // 16 kv rows = two 8-row atoms = 2048 bytes.
+        auto bdesc = [&](int kk) { return sdesc_sw128(vbase + kk * 2048, L::kKVBytes, 1024); };
+        if (kMask == kMaskTrain64 && (live & seen) != 3u) {
+          tc_add_halves<BN / 16>(tO, tP, bdesc, kIdescPV, live, seen);
+        } else {
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          // B = V^T: N = D (contiguous, one 128B swizzle atom), K = kv rows;
-          // 16 kv rows = two 8-row atoms = 2048 bytes.
-          const uint64_t bdesc = sdesc_sw128(vbase + kk * 2048, L::kKVBytes, 1024);
-          tc_mma_ts(tO, tP + kk * 8, bdesc, kIdescPV, (!first || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; ++kk)
+            tc_mma_ts(tO, tP + kk * 8, bdesc(kk), kIdescPV, (!first || kk > 0) ? 1u : 0u);
         }
         tc_commit(bar_pv_full);
         tc_commit(bar_v_empty(sv));
@@ -663,6 +673,9 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!mbar_wait(bar_tile_full(slot), (ti >> 1) & 1, abort_flag, p.status, p.budget_ns)) break;
         const int lin = tile_slot[slot];
         const int n_blk = tile_cnt[slot];  // the MMAs need only the block count
+        // (64-row training mode: the entries too; the softmax threads hold the
+        // slot until the tile's last PV is done)
+        const uint16_t* lst = list_base + slot * p.list_cap + tile_off[slot];
         mbar_arrive(bar_tile_empty(slot));
         ++ti;
         if (lin >= n_total) break;
@@ -670,6 +683,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         ++nq;
         tc_fence_after();
         int j = 0;  // blocks of this tile
+        // halves that list the next block to add, and the one after; halves started
+        uint32_t live = 0u, live_next = 0u, seen = 0u;
+        if constexpr (kMask == kMaskTrain64)
+          if (n_blk > 0) live_next = static_cast<uint32_t>(lst[0]) >> 14;
         bool finished = false;
         while (true) {
           if (j >= n_blk) {
@@ -698,8 +715,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           tc_commit(bar_s_full);
           tc_commit(bar_k_empty(sk));
           if constexpr (kBias) tc_commit(bar_b_empty(jg % kVS));
-          if (j > 0 && !issue_pv(jg - 1, j == 1)) break;
+          if (j > 0 && !issue_pv(jg - 1, j == 1, live, seen)) break;
           ++j;
+          if constexpr (kMask == kMaskTrain64) {
+            seen |= live;
+            live = live_next;
+            if (j < n_blk) live_next = static_cast<uint32_t>(lst[j]) >> 14;
+          }
         }
         // every QK^T of the tile is issued: Q is free once they complete
         tc_commit(bar_q_empty);
@@ -707,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           ok = false;
           break;
         }
-        if (j > 0 && !issue_pv(jbase + j - 1, j == 1)) {
+        if (j > 0 && !issue_pv(jbase + j - 1, j == 1, live, seen)) {
           ok = false;
           break;
         }
@@ -957,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             x = fma2(x, sl2x2, negm2);
             float e0, e1;
             if (exp2_on_fma(e)) {
-              const f2 y = exp2_poly2<kMask == kMaskTrain>(x);
+              const f2 y = exp2_poly2<is_train(kMask)>(x);
               e0 = lo2(y);
               e1 = hi2(y);
             } else {
@@ -1010,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         mx = block_max();
         // a maximum passes over NaN: a row with nothing but NaN (and masked
         // keys) would look like one that sees nothing
-        if constexpr (kMask == kMaskTrain) {
+        if constexpr (is_train(kMask)) {
           if (mx == -INFINITY) {
             float sum = 0.f;
 #pragma unroll
@@ -1071,7 +1093,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                    mbar_wait(bar_pv_full, (jbase + j - 1) & 1, abort_flag, p.status, p.budget_ns));
     if (have_o) tc_fence_after();
     const int qrow = q0 + row;
-    constexpr bool kTrain = kMask == kMaskTrain;
+    constexpr bool kTrain = is_train(kMask);
     const bool empty = kTrain && l_run == 0.f;  // no live key: zeros, log-sum-exp -inf
     const float inv_l = 1.f / l_run;
     // the row's log-sum-exp from a maximum in log2 units and the sum taken against it
@@ -1199,7 +1221,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     named_barrier_sync(1, kThreads);
   }
   // The last CTA to finish resets this launch's tile counters.
-  if (kMask != kMaskTrain && threadIdx.x == 0) {
+  if (!is_train(kMask) && threadIdx.x == 0) {
     __threadfence();
     if (atomicAdd(p.tile_ctr + 1, 1u) == gridDim.x - 1) {
       p.tile_ctr[0] = 0u;
@@ -1296,7 +1318,7 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   if (launch_regs * kThreads < 128 * static_cast<int>(kRegsCtl + kRegsSoftmax)) return SAF_ERR_UNSUPPORTED;
   const int sms = current_device_sms();
   if (sms <= 0) return SAF_ERR_CUDA;
-  if constexpr (kMask != kMaskTrain)
+  if constexpr (!is_train(kMask))
     if ((rc = tile_counter_slot(&p.tile_ctr)) != SAF_OK) return rc;
   p.n_tiles = n_tiles;
   p.BH = p.B * p.H;
@@ -1309,8 +1331,8 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   p.splits = 1;
   if (lead > 0 && kMask != kMaskPool && kMask != kMaskKeys) {
     const int64_t items = static_cast<int64_t>(lead) * p.BH;
-    const int sp = kMask == kMaskTrain ? train_split_cap(items, p.Sk) : split_cap(items, sms);
-    if (kMask == kMaskTrain) {
+    const int sp = is_train(kMask) ? train_split_cap(items, p.Sk) : split_cap(items, sms);
+    if (is_train(kMask)) {
       if (sp > 1 && p.split_part != nullptr) p.splits = sp;
     } else if (sp > 1 && items * sp * kBM * kSplitRow <= kSplitFloats && items * kBM <= kSplitCnts) {
       if ((rc = split_buffers(&p.split_part, &p.split_cnt)) != SAF_OK) return rc;
@@ -1320,7 +1342,7 @@ int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
   }
   const int64_t total = (static_cast<int64_t>(lead) * p.splits + n_tiles - lead) * p.BH;
   int grid = static_cast<int>(total < 2 * sms ? total : 2 * sms);  // two CTAs per SM
-  if constexpr (kMask == kMaskTrain) {
+  if constexpr (is_train(kMask)) {
     // the training forward brings its own buffers, so that its launches may
     // overlap, replays of captured ones included (sized by bsa_train_space)
     if (p.tile_ctr == nullptr) grid = static_cast<int>(total);
@@ -1410,10 +1432,10 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
   const int mask = frames != nullptr ? kMaskFrames
                    : row_ranges != nullptr ? kMaskRanges
                    : pool != nullptr       ? kMaskPool
-                   : train != nullptr      ? kMaskTrain
+                   : train != nullptr      ? (bm == 64 ? kMaskTrain64 : kMaskTrain)
                                            : kMaskNone;
   if (train != nullptr) {
-    if (bias || mask != kMaskTrain) return SAF_ERR_UNSUPPORTED;
+    if (bias || !is_train(mask)) return SAF_ERR_UNSUPPORTED;
     p.lse = train->lse;
     p.split_part = train->split_part;
     p.split_cnt = train->split_cnt;
@@ -1444,9 +1466,13 @@ int32_t bsa_fwd_sm100(const saf_tensor4* q, const saf_tensor4* k, const saf_tens
   SAF_BSA_CASE(64, false, true, kMaskPool)
   SAF_BSA_CASE(64, false, false, kMaskPool)
   SAF_BSA_CASE(128, false, true, kMaskTrain)
+  SAF_BSA_CASE(128, false, true, kMaskTrain64)
   SAF_BSA_CASE(128, false, false, kMaskTrain)
+  SAF_BSA_CASE(128, false, false, kMaskTrain64)
   SAF_BSA_CASE(64, false, true, kMaskTrain)
+  SAF_BSA_CASE(64, false, true, kMaskTrain64)
   SAF_BSA_CASE(64, false, false, kMaskTrain)
+  SAF_BSA_CASE(64, false, false, kMaskTrain64)
 #undef SAF_BSA_CASE
   return SAF_ERR_UNSUPPORTED;
 }

@@ -267,6 +267,31 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same for some rows of D (M = 128): bit 0 of `halves` rows [0, 64), bit 1
+// rows [64, 128); the others are left as they are.
+__device__ __forceinline__ void tc_mma_ts_halves(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                                 uint32_t accumulate, uint32_t halves) {
+  const uint32_t off0 = (halves & 1u) ? 0u : 0xffffffffu, off1 = (halves & 2u) ? 0u : 0xffffffffu;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %6, %6}, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(off0), "r"(off1)
+      : "memory");
+}
+// One A x B product of kSlices K slices of 16 (A: 8 TMEM columns on, B: b_step
+// bytes on) added to the rows of D whose half is in `live`; halves not in
+// `seen` start from zero.  So a half that does not list the other operand's
+// block takes nothing from it, not even 0 times a NaN or an infinity.
+template <int kSlices, class BDesc>
+__device__ __forceinline__ void tc_add_halves(uint32_t d_tmem, uint32_t a_tmem, BDesc b_desc, uint32_t idesc,
+                                              uint32_t live, uint32_t seen) {
+  const uint32_t first = live & ~seen;
+  tc_mma_ts_halves(d_tmem, a_tmem, b_desc(0), idesc, first == 0u ? 1u : 0u, first == 0u ? live : first);
+  if (first != 0u && first != live) tc_mma_ts_halves(d_tmem, a_tmem, b_desc(0), idesc, 1u, live & seen);
+#pragma unroll
+  for (int kk = 1; kk < kSlices; ++kk) tc_mma_ts_halves(d_tmem, a_tmem + kk * 8, b_desc(kk), idesc, 1u, live);
+}
 
 #define SAF_R8(p, i) p[i], p[i + 1], p[i + 2], p[i + 3], p[i + 4], p[i + 5], p[i + 6], p[i + 7]
 

@@ -263,3 +263,37 @@ def test_nan_reaches_every_row_that_sees_it(cuda_device, dtype, bm, S, lead):
     bad = k.clone()
     bad[:, :, S - 1] = float("nan")
     check(q, bad, seen)
+
+
+@pytest.mark.parametrize("bm,bn", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("dtype,H,S,lead", [(BF16, 3, 640, 0), (F16, 2, 640, 0), (F32, 2, 640, 0), (BF16, 1, 4000, 2)])
+def test_values_in_another_blocks_lists(cuda_device, dtype, H, S, lead, bm, bn):
+    """NaN and infinities in a key block that one row block lists, and in that
+    row block's q and dout: what does not see them keeps its bits, 64-row
+    neighbours in the same 128-row tile included."""
+    q, k, v, d = (_randn(280 + i, 1, H, S, 64, dtype=dtype).to(cuda_device) for i in range(4))
+    nbq, nbk = math.ceil(S / bm), math.ceil(S / bn)
+    for row, x, y in ((lead, nbk - 2, 1), (lead + 1, nbk - 1, 0), (nbq - 1, 2, nbk - 1)):
+        mask = _mask(284, 1, H, nbq, nbk, 0.4)
+        mask[:, :, :lead] = True
+        mask[..., x] = mask[:, :, row] = False
+        mask[:, :, row, x] = mask[:, :, row, y] = True
+        csr = kernels.mask_to_csr(mask.to(cuda_device), bm, bn)
+        out, lse = kernels.bsa_fwd_lse(q, k, v, csr, 0.125)
+        clean = kernels.bsa_bwd(d, q, k, v, out, lse, csr, 0.125)
+        rows = torch.zeros(S, dtype=torch.bool, device=cuda_device)
+        rows[row * bm:(row + 1) * bm] = True
+        keys = torch.zeros(S, dtype=torch.bool, device=cuda_device)
+        for c in (x, y):
+            keys[c * bn:(c + 1) * bn] = True
+        q2, k2, v2, d2 = (t.clone() for t in (q, k, v, d))
+        for t, at, value in ((k2, x * bn + 3, "nan"), (v2, x * bn + 9, "inf"), (v2, x * bn + 4, "nan"),
+                             (q2, row * bm + 7, "inf"), (d2, row * bm + 1, "nan"), (d2, row * bm + 2, "inf")):
+            t[:, :, at] = float(value)
+        out2, lse2 = kernels.bsa_fwd_lse(q2, k2, v2, csr, 0.125)
+        dirty = kernels.bsa_bwd(d2, q2, k2, v2, out2, lse2, csr, 0.125)
+        assert torch.equal(out2[:, :, ~rows], out[:, :, ~rows]) and torch.equal(lse2[:, :, ~rows], lse[:, :, ~rows])
+        assert torch.equal(dirty[0][:, :, ~rows], clean[0][:, :, ~rows])
+        assert torch.equal(dirty[1][:, :, ~keys], clean[1][:, :, ~keys])
+        assert torch.equal(dirty[2][:, :, ~keys], clean[2][:, :, ~keys])
+        assert bool(torch.isnan(out2[:, :, row * bm:row * bm + bm]).any()) and bool(torch.isnan(dirty[1][:, :, keys]).any())
