@@ -206,7 +206,7 @@ __device__ void build_lists(const PrepParams& p, int g, int group, bool columns)
           const int64_t entries = p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1) + p.nbq] -
                                   p.row_ptr[static_cast<int64_t>(g) * (p.nbq + 1)];
           const int64_t work = 2 * entries * (p.bm * p.bn) / (128 * 128) * gridDim.x;
-          const int64_t share = max(static_cast<int64_t>(kMinPart), (work + 147) / 148);
+          const int64_t share = max(static_cast<int64_t>(kMinPart), (work + kPlannedSms - 1) / kPlannedSms);
           if (2 * static_cast<int64_t>(tiles) > 3 * share) {
             parts = static_cast<int>(min(static_cast<int64_t>(kMaxParts), (tiles + share - 1) / share));
             slot = atomicAdd(p.w.parts_used, parts);
@@ -424,7 +424,7 @@ constexpr int kSimtSmem = (4 * kT * (D + 4) + 2 * kT * (kT + 4) + 2 * kT) * 4;
 // 424, 378, 376, four heads of 4096 tokens in 128-blocks 727, 625, 592; all of
 // 2 x 1000 tokens 108, 109, 128.
 int simt_chunks(int64_t tiles) {
-  const int64_t want = (8 * 148 + tiles - 1) / tiles;
+  const int64_t want = (8 * kPlannedSms + tiles - 1) / tiles;
   return static_cast<int>(want < 1 ? 1 : want > 8 ? 8 : want);
 }
 

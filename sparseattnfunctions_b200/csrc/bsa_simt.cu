@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(256) bsa_fwd_simt_kernel(const SimtParams p) {
 // they take 54; with eight an SM, 8 heads of 2048 tokens 124 instead of 131 us,
 // but 16 heads of 4096, D = 128, 1692 instead of 1646.
 int simt_chunks(int64_t tiles) {
-  const int64_t want = (4 * 148 + tiles - 1) / tiles;
+  const int64_t want = (4 * kPlannedSms + tiles - 1) / tiles;
   return static_cast<int>(want < 1 ? 1 : want > kMaxChunks ? kMaxChunks : want);
 }
 

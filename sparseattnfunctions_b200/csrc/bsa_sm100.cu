@@ -1281,10 +1281,6 @@ int32_t split_buffers(float** part, int** cnt) {
   return SAF_OK;
 }
 
-// SMs that the training forward's split is sized for (its workspace must not
-// depend on the device that the bytes were asked on).
-constexpr int kTrainSms = 148;
-
 // The most work items one lead tile may be cut into: enough to fill the
 // GPU's CTAs, at most 8.
 int split_cap(int64_t items, int sms) {
@@ -1294,11 +1290,11 @@ int split_cap(int64_t items, int sms) {
 // The training forward splits lead tiles of 25 blocks of 128 keys or more:
 // at two heads, 20 blocks take 31.6 us unsplit and 32.8 split (the counters'
 // clearing and the merge), 33 blocks 47.2 and 35.0, 139 blocks 181 and 60.
-int train_split_cap(int64_t items, int64_t Sk) { return Sk > 24 * 128 ? split_cap(items, kTrainSms) : 1; }
+int train_split_cap(int64_t items, int64_t Sk) { return Sk > 24 * 128 ? split_cap(items, kPlannedSms) : 1; }
 
 // Up to two items an SM the training forward gives each item a CTA of its own
 // and needs no counter (nor its clearing).
-bool train_counts_tiles(int64_t total) { return total > 2 * kTrainSms; }
+bool train_counts_tiles(int64_t total) { return total > 2 * kPlannedSms; }
 
 template <int BN, bool kBias, bool kBF16, int kMask>
 int32_t launch_variant(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,

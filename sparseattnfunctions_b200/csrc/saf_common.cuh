@@ -89,6 +89,11 @@ struct PoolArgs {
   int32_t pool_block;  // 64 or 128 query rows per pooled row
 };
 
+// SMs of a whole B200: what the training kernels divide work by where the
+// division fixes a workspace's size (which is asked for without a device) or the
+// order of a sum (whose bits must not depend on the part of a GPU at hand).
+constexpr int kPlannedSms = 148;
+
 // Training forward of the attention kernels: the row log-sum-exp output
 // [B*H, Sq] and the caller's buffers: partial rows and counters of split tiles
 // (null when every tile runs unsplit), and the 16-bit kernel's next-tile
