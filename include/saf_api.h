@@ -187,8 +187,8 @@ int32_t saf_topk_adaptive_select(const double* in, int32_t is_mass, int64_t BH, 
  * at launch time, and leaves it at zero when it ends: launches ordered on
  * one stream, or fewer than 64 in flight at once, never share a live slot.
  * A launch captured in a CUDA graph keeps its slot for every replay, so a
- * replay must not overlap other attention launches of this library on the
- * same device.
+ * replay must not overlap other attention launches that take slots
+ * (saf_bsa_fwd_lse takes none) on the same device.
  * Replaces: _forward / _fwd_kernel / _fwd_kernel_inner /
  * block_sparse_triton_fn (utils/block_sparse_attn_kernel.py:52-293) and the
  * bias path of MergeAttention.forward (MergeAttention.py:33-49). */

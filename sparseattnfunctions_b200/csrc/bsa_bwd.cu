@@ -59,9 +59,12 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
   w.count_q = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_q) * 4));
   w.count_k = reinterpret_cast<int32_t*>(take(static_cast<size_t>(BH * w.lines_k) * 4));
   if (q->dtype != SAF_F32) {
-    // Cutting pays where one list outlasts an SM's share of the whole.  At
-    // 17776 tokens, a tenth of the blocks and dense text, whole and cut lists
-    // take 232 and 100 us at one head, 245 and 151 at two, 246 and 250 at four.
+    // Cutting pays where one list outlasts an SM's share of the whole.  Whole
+    // and cut lists, a tenth of the 128-blocks and dense text, us: one head of
+    // 17776 tokens 229 and 94; two of 2500, 4000, 17776, 33976 tokens 43 and 41,
+    // 61 and 45, 225 and 139, 423 and 441; three of 4000, 8000, 17776, 33976
+    // tokens 69 and 56, 114 and 79, 225 and 235, 475 and 487; four of 17776
+    // 225 and 236.
     const int64_t longest = (q->S > k->S ? q->S : k->S) / 128;
     w.part_cap = BH <= 3 && 2 * longest > 3 * kMinPart ? kPartCap : 0;
     w.item_cap = static_cast<int>(BH * (w.lines_q + w.lines_k)) + w.part_cap;

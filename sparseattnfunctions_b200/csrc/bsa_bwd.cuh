@@ -9,8 +9,9 @@
 // Every output tile is owned by one work item, which walks its own list of
 // blocks in ascending order: a query tile's key blocks (dq) or a key tile's
 // query blocks (dk, dv).  The products s and dp are formed in both walks
-// (7 matrix products instead of 5), and in return no gradient is accumulated
-// by atomics: equal inputs give equal bits.
+// (7 matrix products instead of 5; the 16-bit kernel runs an eighth, of what
+// rounding takes off dq's ds), and in return no gradient is accumulated by
+// atomics: equal inputs give equal bits.
 #pragma once
 
 #include "saf_common.cuh"

@@ -38,8 +38,9 @@
 // exponent of P), in dk items the largest of the blocks listed for the key's
 // half of the tile, so that a few rows with a large gradient take no bits from
 // the others (with one power for the whole head, rows 2^12 below its largest
-// were left with four bits).  dS then stays
-// below 256 times the largest |v|.
+// were left with four bits).  |do . v - delta| is at most 128 |do| |v|, so dS
+// stays below 256 times the largest |v|: inside f16 for |v| up to 255, and far
+// beyond for values whose signs do not all agree with do's.
 //
 // P and dS are rounded to the 16-bit type because the tensor cores want A and B
 // of one type (walk1 and walk2 are the caller's); the sums over them, S, dP,
@@ -49,16 +50,17 @@
 // rounding does not: with keys whose common part is eight times their spread, dq
 // was off by 3.3 (bf16) and 3.4 to 3.7 (f16) times the output's rounding.  dq
 // therefore adds the product of what the rounding took off too, from P's
-// columns, which its items leave free: 1.0 times.  That costs 2.83 instead of
-// 2.61 ms at the bf16 size below, and 735 instead of 661 us a call at 4 heads of
-// 33976 tokens in f16 (strided).
+// columns, which its items leave free: 1.0 times.  When it was added that cost
+// 2.83 instead of 2.61 ms at the bf16 size below, and 735 instead of 661 us a
+// call at 4 heads of 33976 tokens in f16 (strided).
 //
 // Bound (2 x 30 heads of 17776 tokens, a tenth of the 128-blocks, bf16): the
 // tensor pipe, the exponentials and the issue slots share the SM, none of them
-// full.  2.78 ms at 1965 MHz = 558 TFLOP/s of the five products that the
+// full.  2.69 ms at 1965 MHz = 576 TFLOP/s of the five products that the
 // gradient cannot do without (eight are run: S and dP in both kinds of items,
 // dq in two parts), 3.1 to 3.2 ms once the 1000 W power cap holds the clock lower.
-// Counters at 16 heads: tensor pipe 39 %, MUFU 40 %, issue 45 %, DRAM 8 %.
+// f16, 4 heads of 33976 tokens, strided: 0.64 ms, 536 TFLOP/s.
+// Counters at 16 heads: tensor pipe 41 %, MUFU 41 %, issue 47 %, DRAM 11 %.
 // Before dq's second product, with a part taken out (2.60 ms whole, timing
 // only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
 // products 2.37, no products at all 1.96, no loads of the walked tiles 2.60,

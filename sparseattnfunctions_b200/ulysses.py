@@ -34,6 +34,9 @@ compute stream only where their data is used).
 ``pack`` / ``unpack`` / ``all_to_all`` default to the library kernels and
 ``torch.distributed``; tests inject host versions to check the exchange
 logic with the gloo backend on CPU.
+
+No gradients: the processor is called with ``out=``, so the result is detached
+even when an input requires a gradient.
 """
 from __future__ import annotations
 
