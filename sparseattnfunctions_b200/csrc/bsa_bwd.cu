@@ -69,7 +69,9 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
     w.part_cap = BH <= 3 && 2 * longest > 3 * kMinPart ? kPartCap : 0;
     w.item_cap = static_cast<int>(BH * (w.lines_q + w.lines_k)) + w.part_cap;
     w.items = reinterpret_cast<uint2*>(take(static_cast<size_t>(w.item_cap) * kClasses * 8));
-    w.class_count = reinterpret_cast<int32_t*>(take(kCounters * 4));
+    const int64_t vmax = q->dtype == SAF_F16 ? BH : 0;
+    w.class_count = reinterpret_cast<int32_t*>(take(static_cast<size_t>(kCounters + vmax) * 4));
+    w.vmax = reinterpret_cast<uint32_t*>(w.class_count + kCounters);
     w.next = w.class_count + kClasses;
     w.parts_used = w.next + 1;
     w.split_count = w.next + 2;
@@ -104,8 +106,9 @@ BwdWorkspace layout(const saf_tensor4* q, const saf_tensor4* k, int bm, int bn, 
 struct PrepParams {
   const void* out;
   const void* dout;
-  int64_t o_sb, o_sh, o_ss, d_sb, d_sh, d_ss;
-  int H, Sq, D;
+  const void* v;
+  int64_t o_sb, o_sh, o_ss, d_sb, d_sh, d_ss, v_sb, v_sh, v_ss;
+  int H, Sq, Sk, D;
   const float* lse;
   int64_t lse_stride;  // per head
   float lse_factor, lse_shift;  // stat_lse = lse_shift - lse_factor * lse
@@ -296,7 +299,7 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
       if constexpr (kMax) {
 #pragma unroll
         for (int off = 4; off > 0; off >>= 1) row_max = fmaxf(row_max, __shfl_xor_sync(0xffffffffu, row_max, off));
-        if (sub == 0) p.w.stat_exp[base + row] = static_cast<float>(f16_ds_exponent(row_max));
+        if (sub == 0) p.w.stat_exp[base + row] = static_cast<float>(f16_ds_exponent_do(row_max));
         amax[i / 2] = fmaxf(amax[i / 2], row_max);
       }
     }
@@ -337,6 +340,30 @@ __device__ void row_stats(const PrepParams& p, int g, int chunk) {
   }
 }
 
+// f16: the largest finite |v| of 128 rows of head g (an infinity decides nothing:
+// what sees it is not finite anyway, and the others keep their scale).
+__device__ void value_max(const PrepParams& p, int g, int chunk) {
+  const __half* v = static_cast<const __half*>(p.v) + g / p.H * p.v_sb + g % p.H * p.v_sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint4 x[kRowChunk / 32];
+#pragma unroll
+  for (int i = 0; i < kRowChunk / 32; ++i) {
+    const int row = chunk * kRowChunk + i * 32 + warp * 4 + (lane >> 3);
+    x[i] = row < p.Sk ? *reinterpret_cast<const uint4*>(v + row * p.v_ss + (lane & 7) * 8) : uint4{0, 0, 0, 0};
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRowChunk / 32; ++i)
+#pragma unroll
+    for (const uint32_t w : {x[i].x, x[i].y, x[i].z, x[i].w}) {
+      const float2 f = unpack2(w, static_cast<const __half*>(nullptr));
+      const float a = fabsf(f.x), b = fabsf(f.y);
+      m = fmaxf(m, fmaxf(a < INFINITY ? a : 0.f, b < INFINITY ? b : 0.f));
+    }
+  const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(m));  // non-negative floats order as integers
+  if (lane == 0) atomicMax(p.w.vmax + g, most);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
   const int g = blockIdx.x, x = blockIdx.y;  // every head's lists start before the statistics
@@ -346,8 +373,10 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const PrepParams p) {
     build_lists(p, g, x, true);
   else if (x < p.groups_k + p.groups_q)
     build_lists(p, g, x - p.groups_k, false);
-  else
-    row_stats<T>(p, g, x - p.groups_k - p.groups_q);
+  else if (const int chunk = x - p.groups_k - p.groups_q; chunk < p.w.Sp / kRowChunk)
+    row_stats<T>(p, g, chunk);
+  else if constexpr (std::is_same<T, __half>::value)
+    value_max(p, g, chunk - static_cast<int>(p.w.Sp / kRowChunk));
 }
 
 // ---------------------------------------------------------------------------
@@ -651,7 +680,8 @@ int32_t launch_prep(const PrepParams& p, int BH, cudaStream_t st) {
   const int smem = (kGroup * words + rows + 1) * 4;
   if (smem > 48 * 1024)
     if (const int32_t rc = allow_smem<bwd_prep_kernel<T>>(smem); rc != SAF_OK) return rc;
-  const dim3 grid(static_cast<unsigned>(BH), static_cast<unsigned>(p.groups_k + p.groups_q + p.w.Sp / kRowChunk));
+  const int64_t chunks = p.w.Sp / kRowChunk + (std::is_same<T, __half>::value ? (p.Sk + kRowChunk - 1) / kRowChunk : 0);
+  const dim3 grid(static_cast<unsigned>(BH), static_cast<unsigned>(p.groups_k + p.groups_q + chunks));
   bwd_prep_kernel<T><<<grid, 256, smem, st>>>(p);
   SAF_CUDA_TRY(cudaGetLastError());
   return SAF_OK;
@@ -718,7 +748,9 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
   pp.out = out->data, pp.dout = dout->data;
   pp.o_sb = out->stride_b, pp.o_sh = out->stride_h, pp.o_ss = out->stride_s;
   pp.d_sb = dout->stride_b, pp.d_sh = dout->stride_h, pp.d_ss = dout->stride_s;
-  pp.H = static_cast<int>(q->H), pp.Sq = static_cast<int>(q->S), pp.D = static_cast<int>(q->D);
+  pp.v = v->data, pp.v_sb = v->stride_b, pp.v_sh = v->stride_h, pp.v_ss = v->stride_s;
+  pp.H = static_cast<int>(q->H), pp.D = static_cast<int>(q->D);
+  pp.Sq = static_cast<int>(q->S), pp.Sk = static_cast<int>(k->S);
   pp.lse = lse;
   pp.lse_stride = lse_stride_bh;
   pp.lse_factor = 1.f;
@@ -735,7 +767,8 @@ extern "C" int32_t saf_bsa_bwd(const saf_tensor4* dout, const saf_tensor4* q, co
     pp.lse_factor = kLog2e;
     pp.lse_shift = q->dtype == SAF_F16 ? bwd_f16_p_log2_scale() : 0.f;
     pp.items = 1;
-    SAF_CUDA_TRY(cudaMemsetAsync(pp.w.class_count, 0, kCounters * sizeof(int32_t), st));
+    const size_t counters = kCounters + (q->dtype == SAF_F16 ? BH : 0);  // the value maxima follow them
+    SAF_CUDA_TRY(cudaMemsetAsync(pp.w.class_count, 0, counters * sizeof(int32_t), st));
     rc = q->dtype == SAF_BF16 ? launch_prep<__nv_bfloat16>(pp, BH, st) : launch_prep<__half>(pp, BH, st);
     if (rc != SAF_OK) return rc;
     return bsa_bwd_sm100(dout, q, k, v, dq, dk, dv, block_m, block_n, sm_scale, pp.w, st);

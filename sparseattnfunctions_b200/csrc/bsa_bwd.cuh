@@ -41,10 +41,11 @@ struct BwdWorkspace {
   int32_t* parts_used;
   int32_t* split_count;  // lines cut
   uint2* split;          // [part_cap / 2]: the line as in items, its first part and their number
-  // f16 only: the exponent that takes a row's largest |do| to [2^-4, 2^-3),
-  // and the largest |do| of each 64 rows
+  // f16 only: what a row's largest |do| puts into dS's exponent, the largest
+  // |do| of each 64 rows, and the largest finite |v| of each head
   float* stat_exp;  // [BH, Sp]
   float* amax;      // [BH, Sp / 64]
+  uint32_t* vmax;   // [BH], bits of the float; zeroed with the counters
   float* part;  // partial sums
   // fp32 kernel only: CTAs that share a tile, and the tiles' counts of finished ones
   int chunks;
@@ -54,9 +55,15 @@ struct BwdWorkspace {
   size_t bytes;
 };
 
-// Exponent of the power of two that takes a largest |do| of a to [2^-4, 2^-3);
-// 0 where all are zero or not finite.
-__device__ __forceinline__ int f16_ds_exponent(float a) { return a > 0.f && a <= 65504.f ? -4 - ilogbf(a) : 0; }
+// f16: dS times 2^4 (P's factor) and 2^e stays below 2^15 whatever the signs:
+// |do . v - delta| <= 128 |do| |v| (o is a mean of v), each below twice its
+// power of two, so e = 2 - ilogb(largest |do|) - ilogb(largest |v|).  The two
+// parts of it; 0 where all are zero or not finite.
+__device__ __forceinline__ int f16_exponent(float a) { return a > 0.f && a <= 65504.f ? ilogbf(a) : 0; }
+__device__ __forceinline__ int f16_ds_exponent_do(float a) { return -f16_exponent(a); }
+__device__ __forceinline__ int f16_ds_exponent_v(float a) { return 2 - f16_exponent(a); }
+// 2^e, |e| <= 126
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 // Length classes of the work items: class 15 - floor(log2(blocks)), so that
 // the longest lists start first and the short ones fill the last wave.

@@ -32,15 +32,14 @@
 // TMEM columns: S 128 | dP 128 | P 64 | dS 64 | dv 64 | dk or dq 64.
 //
 // f16: p below 2^-14 and ds of small gradients would leave the type's normal
-// range, so P is formed times 2^4 and dS times a power of two that takes the
-// largest |do| to [2^-4, 2^-3); the outputs are scaled back.  In dq items that
-// is the row's own largest (a row is one thread's, and its power goes into the
+// range, so P is formed times 2^4 and dS times a power of two that keeps it
+// just inside the type for the largest |do| and the head's largest |v|,
+// whatever their signs; the outputs are scaled back.  In dq items that |do| is
+// the row's own largest (a row is one thread's, and its power goes into the
 // exponent of P), in dk items the largest of the blocks listed for the key's
 // half of the tile, so that a few rows with a large gradient take no bits from
 // the others (with one power for the whole head, rows 2^12 below its largest
-// were left with four bits).  |do . v - delta| is at most 128 |do| |v|, so dS
-// stays below 256 times the largest |v|: inside f16 for |v| up to 255, and far
-// beyond for values whose signs do not all agree with do's.
+// were left with four bits).
 //
 // P and dS are rounded to the 16-bit type because the tensor cores want A and B
 // of one type (walk1 and walk2 are the caller's); the sums over them, S, dP,
@@ -112,7 +111,7 @@ struct Item {
   int32_t g, tile;
   int32_t n;     // walked tiles
   int32_t part;  // -1, or where the fp32 sums of this part of a line go
-  int32_t ds_exp[2];  // f16, dk: exponent of dS's power of two for each half of the own tile
+  int32_t ds_exp[2];  // f16: exponent of dS's power of two for each half of the own tile (dq: v's part)
   int32_t pad;
 };
 
@@ -434,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             n = min(n - t0 * per, (t1 - t0) * per);
             im.n = t1 - t0;
           }
+          if (!kBF16) im.ds_exp[0] = im.ds_exp[1] = f16_ds_exponent_v(__uint_as_float(p.w.vmax[im.g]));
           if (!kBF16 && im.keys) {  // the largest |do| of the listed query blocks
             const float* amax = p.w.amax + im.g * (p.w.Sp / kUnit);
             const int per = block / kUnit;
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               a0 = fmaxf(a0, __shfl_xor_sync(0xffffffffu, a0, o));
               a1 = fmaxf(a1, __shfl_xor_sync(0xffffffffu, a1, o));
             }
-            im.ds_exp[0] = f16_ds_exponent(a0);
-            im.ds_exp[1] = f16_ds_exponent(a1);
+            im.ds_exp[0] += f16_ds_exponent_do(a0);
+            im.ds_exp[1] += f16_ds_exponent_do(a1);
           }
         }
         if (lane == 0 && lin < n_items) lin = atomicAdd(p.w.next, 1);  // the next one, in flight over this one
@@ -688,15 +688,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int keys = c.items[slot].keys, n = c.items[slot].n;
       if (keys < 0) break;
       // f16: dS's power of two, for this half of the own tile (dk) or this thread's row (dq)
-      float ds_exp = kBF16 ? 0.f : static_cast<float>(c.items[slot].ds_exp[quarter >> 1]);
+      int ds_exp = kBF16 ? 0 : c.items[slot].ds_exp[quarter >> 1];
       if (keys) {
-        const float ds_scale = kBF16 ? 1.f : exp2f(ds_exp);
+        const float ds_scale = power_of_two(ds_exp);
         for (int j = 0; j < n; ++j, ++t) compute_tile<true, kBF16>(c, p, w, quarter, t, 0.f, 0.f, ds_scale);
       } else {
         const int64_t at = c.items[slot].g * p.w.Sp + c.items[slot].tile * kM + row;
         // dS's power of two goes into the exponent: dq does not need P itself
-        if constexpr (!kBF16) ds_exp = p.w.stat_exp[at];
-        const float nl = p.w.stat_lse[at] + ds_exp;
+        if constexpr (!kBF16) ds_exp += static_cast<int>(p.w.stat_exp[at]);
+        const float nl = p.w.stat_lse[at] + static_cast<float>(ds_exp);
         const float nd = p.w.stat_delta[at];
         for (int j = 0; j < n; ++j, ++t) compute_tile<false, kBF16>(c, p, w, quarter, t, nl, nd, 1.f);
       }
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 32; ++e) r[e] = 0u;
       }
       const float unscale = kBF16 ? 1.f : 1.f / kF16PScale;
-      const float scale = dv ? unscale : kBF16 ? p.scale : p.scale * unscale * exp2f(-ds_exp);
+      const float scale = dv ? unscale : kBF16 ? p.scale : p.scale * unscale * power_of_two(-ds_exp);
       const int part = kParts ? c.items[slot].part : -1;
       if (kParts && part >= 0) {  // sums of a part of the line: fp32, scaled, to the workspace
         if (keys || (w & 1) == 0) {  // dq: one of the two warpgroups that hold the same 32 channels

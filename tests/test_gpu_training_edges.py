@@ -297,3 +297,36 @@ def test_values_in_another_blocks_lists(cuda_device, dtype, H, S, lead, bm, bn):
         assert torch.equal(dirty[1][:, :, ~keys], clean[1][:, :, ~keys])
         assert torch.equal(dirty[2][:, :, ~keys], clean[2][:, :, ~keys])
         assert bool(torch.isnan(out2[:, :, row * bm:row * bm + bm]).any()) and bool(torch.isnan(dirty[1][:, :, keys]).any())
+
+
+@pytest.mark.parametrize("Sk,size", [(2, 4000.0), (2, 60000.0), (70, 60000.0), (300, 3e-6)])
+@pytest.mark.parametrize("bm", [64, 128])
+def test_f16_values_of_any_size(cuda_device, Sk, size, bm):
+    """Values at both ends of f16, all channels of one sign with dout's, so that
+    dout . v is as large as it can be beside them: finite gradients, as exact as
+    for values near 1 (the same tolerances), and infinite where f16 ends."""
+    H, Sq = 2, 200
+    sign = _randn(290, 1, 1, 1, 64).sign()
+    flip = _randn(291, 1, H, Sk, 1).sign()
+    q = _randn(292, 1, H, Sq, 64, dtype=F16)
+    k = _randn(293, 1, H, Sk, 64, dtype=F16, scale=0.05 if size > 1 else 4.0)
+    v = (sign * flip * (0.7 + 0.3 * torch.rand(1, H, Sk, 64, generator=torch.Generator().manual_seed(294))) * size).to(F16)
+    dout = (sign * (0.5 + 0.5 * torch.rand(1, H, Sq, 64, generator=torch.Generator().manual_seed(295))) *
+            (1.0 if size > 1 else 2.0 ** 12)).to(F16)
+    nbq, nbk = math.ceil(Sq / bm), math.ceil(Sk / bm)
+    mask = torch.ones(1, H, nbq, nbk, dtype=torch.bool)
+    csr = kernels.mask_to_csr(mask.to(cuda_device), bm, bm)
+    gq, gk, gv, gd = (t.to(cuda_device) for t in (q, k, v, dout))
+    out, lse = kernels.bsa_fwd_lse(gq, gk, gv, csr, 0.125)
+    grads = kernels.bsa_bwd(gd, gq, gk, gv, out, lse, csr, 0.125)
+    live = otr.token_mask(mask, Sq, Sk, bm, bm)
+    ref = otr.attention_grad(dout, q, k, v, out.cpu(), lse.cpu(), live, 0.125)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        value, by_term, by_size = ref[name]
+        fits = np.abs(value) < 60000.0
+        # one rounding of the result (2^-25 below the normal range), two of each term, fp32 sums
+        tol = U[F16] * np.abs(value) * 1.01 + 2.0 ** -25 + 2 * (U[F16] + 1e-4) * by_term + 4e-5 * by_size
+        off = np.abs(got.double().cpu().numpy() - value)
+        assert fits.any() and bool((off[fits] <= tol[fits]).all()), f"{name}: {np.nanmax(off[fits] / tol[fits])}"
+        past = np.abs(value) > 70000.0
+        assert np.array_equal(got.double().cpu().numpy()[past], np.copysign(np.inf, value[past]))
