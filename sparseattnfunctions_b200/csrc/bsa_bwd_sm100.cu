@@ -58,7 +58,7 @@
 // full.  2.69 ms at 1965 MHz = 576 TFLOP/s of the five products that the
 // gradient cannot do without (eight are run: S and dP in both kinds of items,
 // dq in two parts), 3.1 to 3.2 ms once the 1000 W power cap holds the clock lower.
-// f16, 4 heads of 33976 tokens, strided: 0.64 ms, 536 TFLOP/s.
+// f16, 4 heads of 33976 tokens, strided: 0.62 to 0.64 ms (by box), 536 to 554 TFLOP/s.
 // Counters at 16 heads: tensor pipe 41 %, MUFU 41 %, issue 47 %, DRAM 11 %.
 // Before dq's second product, with a part taken out (2.60 ms whole, timing
 // only): no exponentials 2.24, no S and dP products 2.38, no dv and dk
